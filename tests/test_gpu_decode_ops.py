@@ -1,0 +1,188 @@
+"""What only the kernels of the decode-time ops can get wrong: captured graphs, streams, batch composition, large offsets,
+pages and lengths outside the cache (answered by the kernels' own bounds checks)."""
+
+import pytest
+import torch
+
+from test_decode_ops import BF16, FP16, attention_oracle, check_attention, make_cache, rows_of
+
+from torchtitan_b200.ops import serving
+
+pytestmark = pytest.mark.gpu
+
+
+def _attend(q, k, v, table, n, **kw):
+    return serving.paged_attention_split(q, k, v, table, n, q.shape[-1] ** -0.5, **kw)
+
+
+@pytest.mark.parametrize("D,H,hkv", [(64, 8, 1), (128, 32, 4), (128, 16, 16), (256, 48, 2)])
+def test_a_sequence_gives_the_same_bits_in_every_batch(D, H, hkv):
+    lens = [3000, 1, 700, 40, 1025, 9000]
+    k, v, table, n, _ = make_cache(lens, hkv=hkv, dim=D, page=16, dtype=BF16, device="cuda")
+    q = torch.randn(len(lens), H, D, device="cuda").to(BF16)
+    out, lse = _attend(q, k, v, table, n, return_lse=True)
+    for b in range(len(lens)):
+        one, l1 = _attend(q[b : b + 1], k, v, table[b : b + 1], n[b : b + 1], return_lse=True)
+        assert torch.equal(one[0], out[b]) and torch.equal(l1[0], lse[b])
+    narrow = -(-40 // 16)                                          # a table of its own width
+    assert torch.equal(_attend(q[3:4], k, v, table[3:4, :narrow].contiguous(), n[3:4])[0], out[3])
+
+
+@pytest.mark.parametrize("lens", [[4096 * 16 + 13], [20000, 70000, 5], [128 * 256, 128 * 256 + 1, 128 * 256 - 1]])
+def test_long_sequences(lens):
+    k, v, table, n, _ = make_cache(lens, hkv=2, dim=64, page=64, dtype=BF16, device="cuda")
+    q = (torch.randn(len(lens), 16, 64, device="cuda") * 2).to(BF16)
+    scores = torch.zeros(k.shape[0], 2, 64, device="cuda")
+    out, lse = _attend(q, k, v, table, n, scores=scores, return_lse=True)
+    check_attention(out, attention_oracle(q, k, v, table, n, 0.125), max(lens), 64, BF16, lse, scores, torch.zeros_like(scores), table)
+
+
+def test_offsets_past_32_bits():
+    """A cache of 2^32 + elements: the sequence lies on its last pages."""
+    page, hkv, D = 64, 8, 128
+    pages = (1 << 32) // (page * hkv * D) + 40
+    k = torch.zeros(pages, page, hkv, D, dtype=BF16, device="cuda")
+    v = torch.zeros_like(k)
+    last = torch.arange(pages - 32, pages, device="cuda", dtype=torch.int32)
+    k[-40:].normal_()
+    v[-40:].normal_()
+    n = torch.tensor([32 * page - 5], dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 16, D, device="cuda").to(BF16)
+    scores = torch.zeros(pages, hkv, page, device="cuda")
+    table = last.view(1, -1)
+    out = _attend(q, k, v, table, n, scores=scores)
+    small = torch.arange(32, dtype=torch.int32, device="cuda").view(1, -1)
+    s2 = torch.zeros(32, hkv, page, device="cuda")
+    assert torch.equal(out, _attend(q, k[-32:].clone(), v[-32:].clone(), small, n, scores=s2))
+    assert torch.equal(scores[-32:], s2)
+    fresh = torch.arange(pages - 40, pages - 32, dtype=torch.int32, device="cuda").view(1, -1)
+    lens, kept = serving.kv_cache_evict(k, v, scores, table, n, fresh, 8 * page, 7)
+    for h in range(hkv):
+        idx = kept[0, h].long()
+        want = rows_of(k, last, 32 * page)[idx, h]
+        assert torch.equal(rows_of(k, fresh[0], 8 * page)[:, h], want)
+    del k, v
+
+
+def test_captured_and_replayed():
+    """One graph for attention with weights, eviction and logits; new lengths, tables and logits on every replay. Two graphs
+    replayed in turn, an eager call between them."""
+    lens = [300, 20, 0, 130]
+    k, v, table, n, free = make_cache(lens, hkv=2, dim=128, page=16, dtype=BF16, device="cuda", spare=40, width=32)
+    fresh = free[:16].view(4, 4).to("cuda")
+    q = torch.randn(4, 8, 128, device="cuda").to(BF16)
+    scores = torch.zeros(k.shape[0], 2, 16, device="cuda")
+    x, tok = torch.randn(4, 5003, device="cuda"), torch.randint(0, 5003, (4, 50), device="cuda")
+    tl = torch.tensor([50, 3, 0, 20], dtype=torch.int32, device="cuda")
+
+    def step():
+        out = _attend(q, k, v, table, n, scores=scores)
+        lens, kept = serving.kv_cache_evict(k, v, scores, table, n, fresh, 64, 8)
+        return out, lens, kept, serving.process_logits(x, tok, tl, repetition_penalty=1.2, frequency_penalty=0.1)
+
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = step()
+        graphs.append((g, res))
+    for i, new in enumerate(([300, 20, 0, 130], [17, 0, 4, 1], [512, 500, 1, 16])):
+        new = [min(a, c) for a, c in zip(new, [304, 32, 0, 144])]      # within what was written
+        new = [min(a, b) for a, b in zip(new, lens)]
+        n.copy_(torch.tensor(new, dtype=torch.int32))
+        x.normal_()
+        results = []
+        for g, res in (graphs[i % 2], graphs[(i + 1) % 2], (None, None)):
+            scores.zero_()
+            if g is None:
+                res = step()
+            else:
+                g.replay()
+            results.append([t.clone() for t in (*res, scores)])
+        for r in results[:2]:
+            assert all(torch.equal(a, b) for a, b in zip(r, results[2]))
+
+
+def test_other_streams():
+    """Work on a side stream, with workspaces whose memory the main stream reuses at once."""
+    k, v, table, n, _ = make_cache([5000, 100], hkv=2, dim=128, page=16, dtype=FP16, device="cuda")
+    q = torch.randn(2, 8, 128, device="cuda").to(FP16)
+    x, tok = torch.randn(8, 30011, device="cuda"), torch.randint(0, 30011, (8, 2000), device="cuda")
+    want = _attend(q, k, v, table, n), serving.process_logits(x, tok, presence_penalty=0.5)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            a, b = _attend(q, k, v, table.long(), n.long()), serving.process_logits(x, tok, presence_penalty=0.5)
+        torch.empty(1 << 22, device="cuda").fill_(float("nan"))
+        c = _attend(q, k, v, table, n)
+        side.synchronize()
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1]) and torch.equal(c, want[0])
+
+
+def test_lengths_and_pages_outside_are_not_followed():
+    """The kernels check what the host cannot see: NaN for that sequence, the others untouched by it."""
+    k, v, table, n, free = make_cache([40, 64, 33, 50], hkv=2, dim=64, page=16, dtype=BF16, device="cuda", spare=20)
+    q = torch.randn(4, 4, 64, device="cuda").to(BF16)
+    good = _attend(q, k, v, table, n)
+    bad_t, bad_n = table.clone(), n.clone()
+    bad_t[0, 1], bad_n[2], bad_n[3] = k.shape[0], 65, -1
+    scores = torch.zeros(k.shape[0], 2, 16, device="cuda")
+    out, lse = _attend(q, k, v, bad_t, bad_n, scores=scores, return_lse=True)
+    assert out[[0, 2, 3]].isnan().all() and lse[[0, 2, 3]].isnan().all() and torch.equal(out[1], good[1])
+    bad_t[0, 1] = -5
+    assert _attend(q, k, v, bad_t, n)[0].isnan().all()
+    # beyond the sequence, a table may hold anything
+    wild = torch.full((4, 9), 1 << 30, dtype=torch.int32, device="cuda")
+    wild[:, :4] = table
+    for b, ln in enumerate([40, 64, 33, 50]):
+        wild[b, -(-ln // 16) :] = -7
+    assert torch.equal(_attend(q, k, v, wild, n), good)
+    k0, v0, scores = k.clone(), v.clone(), torch.rand(k.shape[0], 2, 16, device="cuda")
+    fresh = free[:8].view(4, 2).to("cuda")
+    fresh[1, 0] = 1 << 30
+    lens, kept = serving.kv_cache_evict(k, v, scores, bad_t, bad_n, fresh, 32, 4)
+    assert lens.tolist() == [32, 32, 0, 0] and (kept[2:] == -1).all()
+    untouched = torch.ones(k.shape[0], dtype=torch.bool, device="cuda")
+    untouched[fresh[0].long()], untouched[fresh[1, 1].long()] = False, False
+    assert torch.equal(k[untouched].view(torch.int16), k0[untouched].view(torch.int16))
+    assert torch.equal(v[untouched].view(torch.int16), v0[untouched].view(torch.int16))
+    x = torch.randn(2, 100, device="cuda")
+    tok = torch.tensor([[5, 100, -1, 1 << 30], [7, 7, 7, 7]], device="cuda")
+    y = serving.process_logits(x, tok, torch.tensor([99, -3], device="cuda"), presence_penalty=2.0,
+                               bias_ids=torch.tensor([[100, 3], [-9, 1 << 30]], device="cuda"), bias_values=torch.ones(2, 2, device="cuda"))
+    want = x.clone()
+    want[0, 5] -= 2.0
+    want[0, 3] += 1.0
+    assert torch.equal(y, want)
+
+
+def test_layouts_the_kernels_refuse():
+    k, v, table, n, free = make_cache([40], hkv=2, dim=64, page=16, dtype=BF16, device="cuda")
+    q = torch.randn(1, 4, 64, device="cuda").to(BF16)
+    off = torch.zeros(k.numel() + 8, dtype=BF16, device="cuda")[3:][: k.numel()].view(k.shape)
+    for kk in (off, k.transpose(2, 3).contiguous().transpose(2, 3)):
+        with pytest.raises(ValueError, match="16-byte"):
+            _attend(q, kk, v, table, n)
+    odd = torch.zeros(6, 16, 2, 12, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="16 bytes"):
+        serving.kv_cache_evict(odd, odd.clone(), torch.zeros(6, 2, 16, device="cuda"), table, n, free.view(1, -1).to("cuda"), 32)
+
+
+def test_wide_batches_and_vocabularies():
+    """More rows than an axis of a small grid, a vocabulary larger than a cluster holds at once."""
+    B = 5000
+    k, v, table, n, _ = make_cache([1 + i % 3 for i in range(50)], hkv=1, dim=64, page=4, dtype=BF16, device="cuda")
+    q = torch.randn(50, 2, 64, device="cuda").to(BF16)
+    want = _attend(q, k, v, table, n)
+    got = _attend(q.repeat(B // 50, 1, 1), k, v, table.repeat(B // 50, 1), n.repeat(B // 50))
+    assert torch.equal(got, want.repeat(B // 50, 1, 1))
+    V = 1_000_003
+    x = torch.randn(2, V, device="cuda")
+    tok = torch.randint(0, V, (2, 3000), device="cuda")
+    y = serving.process_logits(x, tok, frequency_penalty=0.5)
+    count = torch.zeros(2, V, device="cuda").scatter_add_(1, tok, torch.ones(2, 3000, device="cuda"))
+    assert torch.equal(y, x - 0.5 * count)

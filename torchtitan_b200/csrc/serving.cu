@@ -305,11 +305,18 @@ sample_kernel(const T* __restrict__ logits, const float* __restrict__ uniforms, 
     for (int i = lo; i < hi; ++i) {
       const float v = ld<T>(x, i);
       if (order_key(v) < kmin) continue;
-      last_kept = i;
-      run += __expf((v - gmax) * inv_temp);
+      const float e = __expf((v - gmax) * inv_temp);
+      if (e > 0.f) last_kept = i;      // a token without mass (a masked one) is never drawn
+      run += e;
       if (run > target) { pick = i; break; }
     }
-    if (pick < 0) pick = last_kept >= 0 ? last_kept : hi - 1;
+    if (pick < 0) pick = last_kept;
+    // rounding put the target at the total while this thread's share holds no mass: the last token before it that does
+    for (int i = lo - 1; pick < 0 && i >= 0; --i) {
+      const float v = ld<T>(x, i);
+      if (order_key(v) >= kmin && __expf((v - gmax) * inv_temp) > 0.f) pick = i;
+    }
+    if (pick < 0) pick = hi - 1;
     tokens[row] = pick;
     logprobs[row] = (ld<T>(x, pick) - gmax) - __logf(raw_total);
   }

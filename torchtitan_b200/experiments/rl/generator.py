@@ -49,6 +49,10 @@ class SamplingConfig:
     temperature: float = 0.8
     top_p: float = 0.95
     max_tokens: int = 100
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    """Penalties on tokens that were said before (``ops.serving.process_logits``); the defaults apply none."""
 
 
 class Generator(Configurable):
@@ -65,6 +69,11 @@ class Generator(Configurable):
         kv_block_size: int = 16
         max_kv_blocks: int | None = None
         """Cap on KV-cache blocks; by default ``gpu_memory_limit`` of the free memory is used."""
+        split_decode: bool = False
+        """Decode with attention split over the cache's length (long contexts, small batches)."""
+        cache_budget: int | None = None
+        """Tokens that a sequence keeps in the cache: a longer one is cut back to its most attended and its latest tokens.
+        Changes what the policy computes, so not together with ``batch_invariant_mode``."""
 
         def __post_init__(self):
             assert self.parallelism.data_parallel_shard_degree in (1, -1), (
@@ -77,6 +86,9 @@ class Generator(Configurable):
 
     def __init__(self, config: Config, *, model_spec, model_path: str = "", batch_invariant_mode: bool = False,
                  tokenizer=None, device: torch.device | str | None = None, model=None):
+        if config.cache_budget is not None and batch_invariant_mode:
+            raise ValueError("generator.cache_budget drops cached tokens, which the trainer's recomputation does not: "
+                             "set batch_invariant_mode to False to use it")
         self.config = config
         self.device = torch.device(device) if device is not None else torch.device(
             f"cuda:{torch.cuda.current_device()}" if torch.cuda.is_available() else "cpu")
@@ -99,7 +111,8 @@ class Generator(Configurable):
         self.policy_version = 0
         att = model.config.layer.attention
         n_kv, hd = (att.n_kv_heads or att.n_heads), (att.head_dim or model.config.dim // att.n_heads)
-        per_block = PagedKVCache.bytes_per_block(len(model.layers), config.kv_block_size, n_kv, hd, dtype)
+        per_block = PagedKVCache.bytes_per_block(len(model.layers), config.kv_block_size, n_kv, hd, dtype,
+                                                 with_scores=config.cache_budget is not None)
         if config.max_kv_blocks is not None:
             blocks = config.max_kv_blocks
         elif self.device.type == "cuda":
@@ -111,6 +124,7 @@ class Generator(Configurable):
         self.engine = GenerationEngine(
             self.model, block_size=config.kv_block_size, num_blocks=int(blocks),
             cudagraph=config.compile.cudagraph_mode != "none", eos_id=getattr(tokenizer, "eos_id", None),
+            split_decode=config.split_decode, cache_budget=config.cache_budget,
         )
         self._rng = None
         if config.seed is not None:
@@ -145,7 +159,8 @@ class Generator(Configurable):
         sc = self.config.sampling
         n = self.config.num_samples_per_prompt
         seqs = self.engine.generate(prompts, n_samples=n, max_tokens=sc.max_tokens, temperature=sc.temperature,
-                                    top_p=sc.top_p, generator=self._rng)
+                                    top_p=sc.top_p, generator=self._rng, repetition_penalty=sc.repetition_penalty,
+                                    presence_penalty=sc.presence_penalty, frequency_penalty=sc.frequency_penalty)
         eps = []
         for s in seqs:
             ids = s.tokens[:-1] if s.hit_eos else s.tokens

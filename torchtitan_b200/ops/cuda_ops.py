@@ -11,6 +11,8 @@ so once in the log.
 
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
 
 import torch
@@ -992,6 +994,108 @@ def paged_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tens
     cl = context_lens if context_lens.dtype == torch.int32 else context_lens.to(torch.int32)
     _ck(_lib().tt_paged_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), bt.contiguous().data_ptr(), cl.data_ptr(),
                                out.data_ptr(), float(scale), B, H, Hkv, D, bs, bt.shape[1], _stream()), "tt_paged_decode")
+    return out
+
+
+PAGED_SPLIT_DIMS = (64, 128, 256)
+
+
+def _i32(t: Tensor) -> Tensor:
+    return t if t.dtype == torch.int32 else t.to(torch.int32)
+
+
+def _rows_i32(t: Tensor) -> Tensor:
+    t = _i32(t)
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _cache_strides(name: str, t: Tensor, unit: int) -> list:
+    """(page, token, head) strides in units of ``unit`` bytes of a cache whose heads are contiguous on 16-byte boundaries."""
+    size = t.element_size()
+    strides = [t.stride(i) * size if t.shape[i] > 1 else 0 for i in range(3)]
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 16 for s in strides):
+        raise ValueError(f"{name} cache: heads must be contiguous and start on 16-byte boundaries (strides {t.stride()})")
+    return [s // unit for s in strides]
+
+
+def paged_split(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tensor, context_lens: Tensor, scale: float, window, sinks,
+                scores, return_lse: bool):
+    """``serving.paged_attention_split`` on the kernels of csrc/paged_split.cu (arguments checked there)."""
+    B, H, D = q.shape
+    nb, bs, Hkv, _ = k_cache.shape
+    with torch.cuda.device(q.device):
+        if q.stride(2) != 1:
+            q = q.contiguous()
+        size = k_cache.element_size()
+        bt, cl = _rows_i32(block_tables), _i32(context_lens).contiguous()
+        if sinks is not None:
+            sinks = sinks.to(torch.float32).contiguous()
+        L = _lib()
+        room = bt.shape[1] * bs
+        win = 0 if window is None else min(int(window), room)
+        if win >= room:
+            win = 0
+        span = min(room, win + 15) if win else room
+        chunks = L.tt_paged_split_chunks(room, win)
+        new = functools.partial(torch.empty, dtype=torch.float32, device=q.device)
+        out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
+        lse = new((B, H)) if return_lse else None
+        ws_o, ws_ml = new((B, chunks, H, D)), new((B, chunks, H, 2))
+        ws_tot, ws_x = (new((B, H, 2)), new((B, H, span))) if scores is not None else (None, None)
+        strides = (ctypes.c_longlong * 9)(q.stride(0), q.stride(1), *_cache_strides("key", k_cache, size),
+                                          *_cache_strides("value", v_cache, size), bt.stride(0))
+        _ck(L.tt_paged_split(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), bt.data_ptr(), cl.data_ptr(), out.data_ptr(),
+                             _p(lse), _p(sinks), _p(scores), ws_o.data_ptr(), ws_ml.data_ptr(), _p(ws_tot), _p(ws_x), strides,
+                             B, H, Hkv, D, bs, bt.shape[1], nb, win, span, chunks, float(scale),
+                             0 if q.dtype == torch.bfloat16 else 2, _stream()), "tt_paged_split")
+    return (out, lse) if return_lse else out
+
+
+def kv_evict(k_cache: Tensor, v_cache: Tensor, scores: Tensor, block_tables: Tensor, context_lens: Tensor, new_tables: Tensor,
+             keep: int, recent: int):
+    """``serving.kv_cache_evict`` on the kernels of csrc/kv_evict.cu (arguments checked there)."""
+    B = block_tables.shape[0]
+    nb, bs, Hkv, D = k_cache.shape
+    row = D * k_cache.element_size()
+    if row % 16:
+        raise ValueError(f"kv_cache_evict moves rows of multiples of 16 bytes, got head_dim {D} of {k_cache.dtype}")
+    with torch.cuda.device(k_cache.device):
+        bt, cl, nt = _rows_i32(block_tables), _i32(context_lens).contiguous(), _rows_i32(new_tables)
+        lens = torch.empty(B, dtype=torch.int32, device=k_cache.device)
+        kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=k_cache.device)
+        strides = (ctypes.c_longlong * 8)(*_cache_strides("key", k_cache, 1), *_cache_strides("value", v_cache, 1), bt.stride(0),
+                                          nt.stride(0))
+        _ck(_lib().tt_kv_evict(k_cache.data_ptr(), v_cache.data_ptr(), scores.data_ptr(), bt.data_ptr(), cl.data_ptr(), nt.data_ptr(),
+                               lens.data_ptr(), kept.data_ptr(), strides, B, Hkv, bs, bt.shape[1], nt.shape[1], nb, row, keep, recent,
+                               _stream()), "tt_kv_evict")
+    return lens, kept
+
+
+def adjust_logits(logits: Tensor, tokens, lens, prompt_lens, rep, pres, freq, bias_ids, bias_values, allowed, out) -> Tensor:
+    """``serving.process_logits`` on the kernels of csrc/logits.cu (arguments checked there)."""
+    B, V = logits.shape
+    with torch.cuda.device(logits.device):
+        if logits.stride(1) != 1:
+            logits = logits.contiguous()
+        if out is None:
+            out = torch.empty((B, V), dtype=logits.dtype, device=logits.device)
+        if tokens is not None and tokens.stride(-1) != 1 and tokens.shape[1] > 1:
+            tokens = tokens.contiguous()
+        # the converted forms are bound to names: they must outlive the launch
+        cl = None if lens is None else _i32(lens).contiguous()
+        cp = None if prompt_lens is None else _i32(prompt_lens).contiguous()
+        ids = None if bias_ids is None else _rows_i32(bias_ids)
+        vals = bias_values if bias_values is None or bias_values.stride(-1) == 1 else bias_values.contiguous()
+        mask = allowed if allowed is None or allowed.stride(-1) == 1 else allowed.contiguous()
+        per_row = [p.contiguous() if torch.is_tensor(p) else None for p in (rep, pres, freq)]
+        value = [0.0 if torch.is_tensor(p) else float(p) for p in (rep, pres, freq)]
+        row = lambda t: 0 if t is None else t.stride(0)  # noqa: E731
+        strides = (ctypes.c_longlong * 6)(logits.stride(0), out.stride(0), row(tokens), row(ids), row(vals), row(mask))
+        _ck(_lib().tt_process_logits(logits.data_ptr(), out.data_ptr(), _p(tokens), int(tokens is not None and tokens.dtype == torch.int64),
+                                     _p(cl), _p(cp), *(_p(p) for p in per_row), *value, _p(ids), _p(vals),
+                                     0 if ids is None else ids.shape[1], _p(mask), strides, B, V,
+                                     0 if tokens is None else tokens.shape[1],
+                                     {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}[logits.dtype], _stream()), "tt_process_logits")
     return out
 
 
