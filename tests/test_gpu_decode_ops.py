@@ -186,3 +186,10 @@ def test_wide_batches_and_vocabularies():
     y = serving.process_logits(x, tok, frequency_penalty=0.5)
     count = torch.zeros(2, V, device="cuda").scatter_add_(1, tok, torch.ones(2, 3000, device="cuda"))
     assert torch.equal(y, x - 0.5 * count)
+
+
+def test_queries_on_odd_addresses():
+    k, v, table, n, _ = make_cache([70, 9], hkv=2, dim=64, page=16, dtype=BF16, device="cuda")
+    wide = torch.randn(2, 4 * 65 + 1, device="cuda").to(BF16)
+    q = wide[:, 1:].view(2, 4, 65)[..., :64]
+    assert torch.equal(_attend(q, k, v, table, n), _attend(q.clone(), k, v, table, n))

@@ -23,7 +23,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMinChunk = 256;    // tokens
 constexpr int kMaxChunks = 128;   // per sequence: bounds the workspace and the join's work
-constexpr int kTile = 8;          // query heads of one kv head that a CTA takes together
+constexpr int kTile = 8;          // query heads of one kv head in a tile of columns
+constexpr int kMaxBatch = 4096;   // sequences of one launch (their chunk counts are kept in shared memory)
 
 struct Args {
   const void *q, *k, *v;
@@ -73,108 +74,394 @@ __device__ __forceinline__ int page_of(const Args& a, int b, int t) {
   return p >= 0 && p < a.pages ? p : -1;
 }
 
-// CTA = (chunk, kv head and tile of its query heads, sequence). A warp takes every fourth token; a lane holds D / 32 dims.
+// The end of a query head: sink, division, output. top, sum, x: maximum, sum and weighted values over all of its tokens.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) split_kernel(const Args a) {
-  constexpr int E = D / 32;
-  const int c = blockIdx.x, tiles = gridDim.y / a.Hkv, hk = blockIdx.y / tiles, b = blockIdx.z;
-  const int G = a.H / a.Hkv, g0 = (blockIdx.y % tiles) * kTile, ng = min(kTile, G - g0);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const Range r = range_of(a, b);
-  const int len = chunk_len(r.n - r.lo), t0 = r.lo + c * len, t1 = min(r.n, t0 + len);
-  if (t0 >= t1) return;
-  __shared__ float s_o[4][kTile][D];
-  __shared__ float2 s_ml[4][kTile];
-  float qf[kTile][E], acc[kTile][E], m[kTile], l[kTile];
-#pragma unroll
-  for (int g = 0; g < kTile; ++g) {
-    m[g] = -INFINITY;
-    l[g] = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      acc[g][e] = 0.f;
-      qf[g][e] = g < ng ? to_f(static_cast<const T*>(a.q)[b * a.q_b + (hk * G + g0 + g) * a.q_h + lane * E + e]) : 0.f;
-    }
+__device__ __forceinline__ void finish(const Args& a, int b, int h, int d, float top, float sum, float x) {
+  const long long bh = static_cast<long long>(b) * a.H + h;
+  if (a.sinks) {
+    const float sink = a.sinks[h] * kLog2e, all = fmaxf(top, sink), base = all == -INFINITY ? 0.f : all;
+    const float f = exp2f(top - base);
+    x *= f;
+    sum = sum * f + exp2f(sink - base);
+    top = all;
   }
-  for (int t = t0 + warp; t < t1; t += 4) {
-    if (t < r.first) continue;
-    const int p = page_of(a, b, t);
-    const T* kp = static_cast<const T*>(a.k) + max(p, 0) * a.k_page + (t % a.page) * a.k_tok + hk * a.k_head + lane * E;
-    const T* vp = static_cast<const T*>(a.v) + max(p, 0) * a.v_page + (t % a.page) * a.v_tok + hk * a.v_head + lane * E;
-    float kf[E], vf[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      kf[e] = to_f(kp[e]);
-      vf[e] = to_f(vp[e]);
-    }
-#pragma unroll
-    for (int g = 0; g < kTile; ++g) {
-      float x = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) x += qf[g][e] * kf[e];
-      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-      x = p < 0 ? NAN : x * a.scale * kLog2e;
-      if (a.ws_x && lane == 0 && g < ng)
-        a.ws_x[((static_cast<long long>(b) * a.Hkv + hk) * a.span + (t - r.lo)) * G + g0 + g] = x;
-      const float top = fmaxf(m[g], x);
-      const float f = top == -INFINITY ? 0.f : exp2f(m[g] - top), w = x == -INFINITY ? 0.f : exp2f(x - top);
-      m[g] = top;
-      l[g] = l[g] * f + w;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[g][e] = acc[g][e] * f + w * vf[e];
-    }
-  }
-#pragma unroll
-  for (int g = 0; g < kTile; ++g) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) s_o[warp][g][lane * E + e] = acc[g][e];
-    if (lane == 0) s_ml[warp][g] = make_float2(m[g], l[g]);
-  }
-  __syncthreads();
-  const long long row = (static_cast<long long>(b) * a.chunks + c) * a.H + hk * G + g0;
-  for (int i = threadIdx.x; i < ng * D; i += 128) {
-    const int g = i / D, d = i % D;
-    float top = -INFINITY, sum = 0.f, o = 0.f;
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, s_ml[w][g].x);
-    for (int w = 0; w < 4; ++w) {
-      const float f = s_ml[w][g].x == -INFINITY ? 0.f : exp2f(s_ml[w][g].x - top);
-      // a warp whose tokens all gave NaN has m = -inf but a NaN sum: the sum is taken whole
-      sum += s_ml[w][g].x == -INFINITY ? s_ml[w][g].y : s_ml[w][g].y * f;
-      o += s_ml[w][g].x == -INFINITY ? s_o[w][g][d] : s_o[w][g][d] * f;
-    }
-    a.ws_o[(row + g) * D + d] = o;
-    if (d == 0) a.ws_ml[row + g] = make_float2(top, sum);
+  static_cast<T*>(a.out)[bh * D + d] = from_f<T>(sum == 0.f ? 0.f : x / sum);
+  if (d == 0) {
+    if (a.lse) a.lse[bh] = (top + log2f(sum)) * kLn2;
+    if (a.ws_tot) a.ws_tot[bh] = make_float2(top, sum);
   }
 }
 
-// CTA = (query head, sequence).
+// ---- pieces of the matrix path
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {   // zeros where !ok (src is not read then)
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_group() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <typename T> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// (lower half, upper half) rounded to T
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+
+constexpr int kWarps = 4;
+constexpr int kRows = 16;        // tokens of one step of a warp
+
+constexpr int kPitch = 64 + 4;   // merged values are passed on 64 dims at a time, rows 4 banks apart
+
+template <int D> struct Ring {
+  static constexpr int kRowBytes = 2 * D, kStageBytes = 2 * kRows * kRowBytes;     // K rows, then V rows
+  static constexpr int kStages = D == 64 ? 6 : 3;
+  static constexpr int kBytes = kWarps * kStages * kStageBytes;
+};
+template <int D, int NT> constexpr int smem_bytes() {
+  return Ring<D>::kBytes + kWarps * kTile * kPitch * 4 + kWarps * kTile * NT * 8 + (D == 256 ? NT * (D / 16) * 32 * 8 : 0);
+}
+
+// One piece of work: chunk c of sequence b for head tile hkt (kv head x tile of NT * 8 query heads).
+struct Item {
+  int b, c, hkt, t0, t1, chunks;
+  Range r;
+};
+
+// items are numbered ((sequence, chunk), head tile), head tile fastest: neighbours read the same tokens' heads, which lie
+// next to each other in the cache.
+__device__ __forceinline__ void item_at(Item& it, const Args& a, const int* first_chunk, int hkts, int i) {
+  const int bc = i / hkts;
+  it.hkt = i - bc * hkts;
+  int lo = 0, hi = a.B - 1;                       // the last sequence that begins at or before bc
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first_chunk[mid] <= bc) lo = mid; else hi = mid - 1;
+  }
+  it.b = lo;
+  it.c = bc - first_chunk[lo];
+  it.chunks = first_chunk[lo + 1] - first_chunk[lo];
+  it.r = range_of(a, lo);
+  const int len = chunk_len(it.r.n - it.r.lo);
+  it.t0 = it.r.lo + it.c * len;
+  it.t1 = min(it.r.n, it.t0 + len);
+}
+
+// Tokens as rows of the products' left operand, query heads as columns: S^T = K q^T and O^T += V^T P^T, eight query heads
+// being one tile of columns, so that groups of up to 8 heads waste nothing. P is passed as its rounding to T plus the
+// rounding of the remainder, which keeps 16 bits of it (P in T alone would add an error as large as the output's own
+// rounding). A warp owns every fourth 16 tokens of a chunk and a ring of stages; its loads run ahead across chunks.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
+  using R = Ring<D>;
+  constexpr int CH = D / 8;                       // 16-byte pieces of a row
+  constexpr bool QS = D == 256;                   // q's fragments in shared memory: they do not fit the registers
+  extern __shared__ __align__(128) unsigned char smem[];
+  float* s_o = reinterpret_cast<float*>(smem + R::kBytes);                                   // [warp][8][kPitch]
+  float2* s_ml = reinterpret_cast<float2*>(s_o + kWarps * kTile * kPitch);                  // [warp][NT * 8]
+  uint2* s_q = reinterpret_cast<uint2*>(s_ml + kWarps * kTile * NT);                         // [NT][D / 16][32]
+  int* first_chunk = reinterpret_cast<int*>(s_q + (QS ? NT * (D / 16) * 32 : 0));            // [B + 1]
+  __shared__ int s_sum[kWarps];
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int G = a.H / a.Hkv, tiles = (G + kTile * NT - 1) / (kTile * NT), hkts = a.Hkv * tiles;
+
+  // prefix sums of the sequences' chunk counts
+  {
+    const int per = (a.B + 32 * kWarps - 1) / (32 * kWarps), b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      const Range r = range_of(a, b);
+      const int n = r.n - r.lo;
+      first_chunk[b] = sum;
+      if (n > 0) sum += (n + chunk_len(n) - 1) / chunk_len(n);
+    }
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (lane == 31) s_sum[warp] = inc;
+    __syncthreads();
+    int before = inc - sum;
+    for (int w = 0; w < warp; ++w) before += s_sum[w];
+    for (int b = b0; b < b1; ++b) first_chunk[b] += before;
+    if (tid == 32 * kWarps - 1) first_chunk[a.B] = before + sum;
+    __syncthreads();
+  }
+  const int items = first_chunk[a.B] * hkts;
+  const uint32_t ring = smem_u32(smem) + warp * R::kStages * R::kStageBytes;
+  const T* kc = static_cast<const T*>(a.k);
+  const T* vc = static_cast<const T*>(a.v);
+
+  // ---- the loads: `head` is the item being loaded, ht its next token, page its table entry for row lane % 16
+  Item head;
+  int hi = blockIdx.x, ht = 0, page = -1, slot = 0;
+  auto look_up = [&]() {                          // the table entry of the step at ht, ahead of its use
+    const int t = ht + (lane & 15);
+    const bool live = t >= head.r.first && t < head.t1;
+    const int at = live ? t / a.page : 0;
+    slot = t - at * a.page;
+    page = live ? a.tables[head.b * a.table_row + at] : -1;
+    if (live && (page < 0 || page >= a.pages)) page = -2;         // named outside the cache
+  };
+  auto settle = [&]() {                           // the first step at or after (hi, ht) that this warp has
+    while (hi < items && ht >= head.t1) {
+      hi += gridDim.x;
+      if (hi < items) {
+        item_at(head, a, first_chunk, hkts, hi);
+        ht = head.t0 + warp * kRows;
+      }
+    }
+    if (hi < items) look_up();
+  };
+  if (hi < items) {
+    item_at(head, a, first_chunk, hkts, hi);
+    ht = head.t0 + warp * kRows;
+    settle();
+  }
+  auto load = [&](int stage) {                    // one commit group, empty when nothing is left
+    if (hi < items) {
+      const uint32_t dst = ring + stage * R::kStageBytes;
+      const int hk = head.hkt / tiles;
+#pragma unroll
+      for (int i = 0; i < CH / 2; ++i) {
+        const int idx = i * 32 + lane, row = idx / CH, ch = idx % CH;
+        const int p = __shfl_sync(0xffffffffu, page, row), s = __shfl_sync(0xffffffffu, slot, row);
+        const bool ok = p >= 0;
+        const uint32_t at = row * R::kRowBytes + ((ch ^ (row & 7)) << 4);
+        const T* ks = ok ? kc + p * a.k_page + s * a.k_tok + hk * a.k_head + ch * 8 : kc;
+        const T* vs = ok ? vc + p * a.v_page + s * a.v_tok + hk * a.v_head + ch * 8 : vc;
+        if (p == -2) {
+          // a bad page number: a key of NaNs, which makes the whole sequence NaN
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + at), "r"(0x7fff7fffu) : "memory");
+        } else {
+          copy16(dst + at, ks, ok);
+        }
+        copy16(dst + kRows * R::kRowBytes + at, vs, ok);
+      }
+      ht += kWarps * kRows;
+      settle();
+    }
+    commit();
+  };
+#pragma unroll
+  for (int s = 0; s < R::kStages - 1; ++s) load(s);
+  int stage = 0;
+
+  const float c2 = a.scale * kLog2e;
+  const int cx = 2 * (lane & 3);                  // this thread's columns (heads): cx, cx + 1 of each tile
+  Item it;
+  for (int i = blockIdx.x; i < items; i += gridDim.x) {
+    item_at(it, a, first_chunk, hkts, i);
+    const int hk = it.hkt / tiles, g0 = (it.hkt % tiles) * kTile * NT, ng = min(kTile * NT, G - g0);
+    // q as the right operand: column = head, consecutive k in a register
+    uint2 qf[QS ? 1 : NT][QS ? 1 : D / 16];
+    auto q_frag = [&](int nt, int kk) {
+      const int g = nt * kTile + lane / 4;
+      uint2 v = make_uint2(0, 0);
+      if (g < ng) {
+        const T* qp = static_cast<const T*>(a.q) + it.b * a.q_b + (hk * G + g0 + g) * a.q_h + kk * 16 + cx;
+        v.x = *reinterpret_cast<const uint32_t*>(qp);
+        v.y = *reinterpret_cast<const uint32_t*>(qp + 8);
+      }
+      return v;
+    };
+    if constexpr (QS) {
+      __syncthreads();
+      for (int f = warp; f < NT * (D / 16); f += kWarps) s_q[f * 32 + lane] = q_frag(f / (D / 16), f % (D / 16));
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) qf[nt][kk] = q_frag(nt, kk);
+    }
+    float o[NT][D / 16][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int dd = 0; dd < D / 16; ++dd)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][dd][e] = 0.f;
+    }
+    for (int t = it.t0 + warp * kRows; t < it.t1; t += kWarps * kRows) {
+      load(stage == 0 ? R::kStages - 1 : stage - 1);
+      wait_group<R::kStages - 1>();
+      __syncwarp();
+      const uint32_t ks = ring + stage * R::kStageBytes, vs = ks + kRows * R::kRowBytes;
+      float s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      {
+        const int row = lane & 15, half = lane >> 4;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t kf[4];
+          ldm4(kf, ks + row * R::kRowBytes + (((kk * 2 + half) ^ (row & 7)) << 4));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            uint2 qv;
+            if constexpr (QS) qv = s_q[(nt * (D / 16) + kk) * 32 + lane]; else qv = qf[nt][kk];
+            mma<T>(s[nt], kf, qv.x, qv.y);
+          }
+        }
+      }
+      const int ta = t + lane / 4, tb = ta + 8;
+      const bool la = ta >= it.r.first && ta < it.t1, lb = tb >= it.r.first && tb < it.t1;
+      uint32_t hi_p[NT][2], lo_p[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] = (e < 2 ? la : lb) ? s[nt][e] * c2 : -INFINITY;
+        if (a.ws_x) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int g = nt * kTile + cx + (e & 1), tt = e < 2 ? ta : tb;
+            if (g < ng && (e < 2 ? la : lb)) a.ws_x[((static_cast<long long>(it.b) * a.Hkv + hk) * a.span + (tt - it.r.lo)) * G + g0 + g] = s[nt][e];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = fmaxf(s[nt][e], s[nt][e + 2]);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          top = fmaxf(top, m[nt][e]);
+          const float base = top == -INFINITY ? 0.f : top, f = exp2f(m[nt][e] - base);
+          m[nt][e] = top;
+          s[nt][e] = exp2f(s[nt][e] - base);
+          s[nt][e + 2] = exp2f(s[nt][e + 2] - base);
+          l[nt][e] = l[nt][e] * f + s[nt][e] + s[nt][e + 2];
+#pragma unroll
+          for (int dd = 0; dd < D / 16; ++dd) {
+            o[nt][dd][e] *= f;
+            o[nt][dd][e + 2] *= f;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t top = pack2<T>(s[nt][2 * h], s[nt][2 * h + 1]);
+          const float2 back = unpack2<T>(top);
+          hi_p[nt][h] = transpose8(top);
+          lo_p[nt][h] = transpose8(pack2<T>(s[nt][2 * h] - back.x, s[nt][2 * h + 1] - back.y));
+        }
+      }
+      {
+        const int row = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+#pragma unroll
+        for (int dd = 0; dd < D / 16; ++dd) {
+          uint32_t vf[4];
+          ldm4t(vf, vs + row * R::kRowBytes + (((dd * 2 + half) ^ (row & 7)) << 4));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma<T>(o[nt][dd], vf, hi_p[nt][0], hi_p[nt][1]);
+            mma<T>(o[nt][dd], vf, lo_p[nt][0], lo_p[nt][1]);
+          }
+        }
+      }
+      __syncwarp();                               // before the stage is filled again
+      stage = stage + 1 == R::kStages ? 0 : stage + 1;
+    }
+
+    // ---- the four warps' parts, in their order
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[nt][e];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        if (lane < 4) s_ml[warp * kTile * NT + nt * kTile + cx + e] = make_float2(m[nt][e], x);
+      }
+    const long long row = static_cast<long long>(it.b) * a.chunks * a.H + static_cast<long long>(it.c) * a.H + hk * G + g0;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int part = 0; part < D / 64; ++part) {
+        float* mine = s_o + warp * kTile * kPitch;
+#pragma unroll
+        for (int dd = 0; dd < 4; ++dd)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mine[(cx + (e & 1)) * kPitch + dd * 16 + lane / 4 + (e >> 1) * 8] = o[nt][part * 4 + dd][e];
+        __syncthreads();
+        for (int j = tid; j < kTile * 64; j += 32 * kWarps) {
+          const int g = j / 64, d = j % 64, gg = nt * kTile + g;
+          if (gg >= ng) break;
+          float top = -INFINITY, sum = 0.f, x = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w * kTile * NT + gg].x);
+          const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float2 y = s_ml[w * kTile * NT + gg];
+            // NaN tokens leave m alone: a warp that saw nothing else has m = -inf and a NaN sum, which 0 * NaN carries on
+            const float f = exp2f(y.x - base);
+            sum += y.y * f;
+            x += s_o[(w * kTile + g) * kPitch + d] * f;
+          }
+          const int at = part * 64 + d;
+          if (it.chunks > 1) {
+            a.ws_o[(row + gg) * D + at] = x;
+            if (at == 0) a.ws_ml[row + gg] = make_float2(top, sum);
+          } else {
+            finish<T, D>(a, it.b, hk * G + g0 + gg, at, top, sum, x);
+          }
+        }
+        __syncthreads();
+      }
+    }
+  }
+}
+
+// CTA = (query head, sequence): the chunks in their order.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const Args a) {
   const int h = blockIdx.x, b = blockIdx.y;
   const Range r = range_of(a, b);
   const int span = r.n - r.lo, nc = span > 0 ? (span + chunk_len(span) - 1) / chunk_len(span) : 0;
+  if (nc == 1) return;                             // written by the split kernel
   const float2* ml = a.ws_ml + static_cast<long long>(b) * a.chunks * a.H + h;
   const float* po = a.ws_o + (static_cast<long long>(b) * a.chunks * a.H + h) * D;
-  const float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
-  float top = sink;
+  float top = -INFINITY, sum = r.bad ? NAN : 0.f;
   for (int c = 0; c < nc; ++c) top = fmaxf(top, ml[static_cast<long long>(c) * a.H].x);
-  float sum = sink == -INFINITY ? 0.f : exp2f(sink - top);
+  const float base = top == -INFINITY ? 0.f : top;
   for (int c = 0; c < nc; ++c) {
     const float2 x = ml[static_cast<long long>(c) * a.H];
-    sum += x.x == -INFINITY ? x.y : x.y * exp2f(x.x - top);
+    sum += x.y * exp2f(x.x - base);
   }
-  if (r.bad) sum = NAN;
   for (int d = threadIdx.x; d < D; d += 128) {
     float o = 0.f;
-    for (int c = 0; c < nc; ++c) {
-      const float mc = ml[static_cast<long long>(c) * a.H].x, x = po[static_cast<long long>(c) * a.H * D + d];
-      o += mc == -INFINITY ? x : x * exp2f(mc - top);
-    }
-    static_cast<T*>(a.out)[(static_cast<long long>(b) * a.H + h) * D + d] = from_f<T>(sum == 0.f ? 0.f : o / sum);
-  }
-  if (threadIdx.x == 0) {
-    if (a.lse) a.lse[static_cast<long long>(b) * a.H + h] = (top + log2f(sum)) * kLn2;
-    if (a.ws_tot) a.ws_tot[static_cast<long long>(b) * a.H + h] = make_float2(top, sum);
+    for (int c = 0; c < nc; ++c) o += po[static_cast<long long>(c) * a.H * D + d] * exp2f(ml[static_cast<long long>(c) * a.H].x - base);
+    finish<T, D>(a, b, h, d, top, sum, o);
   }
 }
 
@@ -195,10 +482,18 @@ __global__ void __launch_bounds__(128) score_kernel(const Args a) {
   }
 }
 
-template <typename T, int D>
-int launch(const Args& a, cudaStream_t st) {
-  const int G = a.H / a.Hkv, tiles = (G + kTile - 1) / kTile;
-  if (a.chunks > 0) split_kernel<T, D><<<dim3(a.chunks, a.Hkv * tiles, a.B), 128, 0, st>>>(a);
+template <typename T, int D, int NT>
+int launch(const Args& a, int sms, cudaStream_t st) {
+  const int G = a.H / a.Hkv, tiles = (G + kTile * NT - 1) / (kTile * NT);
+  if (a.chunks > 0) {
+    const int bytes = smem_bytes<D, NT>() + (a.B + 1) * 4;
+    if (bytes > 227 * 1024) return -2;
+    if (cudaFuncSetAttribute(split_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -4;
+    const long long most = static_cast<long long>(a.B) * a.chunks * a.Hkv * tiles;
+    const int per_sm = 228 * 1024 / (bytes + 1024);
+    const long long grid = static_cast<long long>(sms) * (per_sm > 0 ? per_sm : 1);
+    split_kernel<T, D, NT><<<static_cast<unsigned>(most < grid ? most : grid), 32 * kWarps, bytes, st>>>(a);
+  }
   join_kernel<T, D><<<dim3(a.H, a.B), 128, 0, st>>>(a);
   if (a.scores && a.chunks > 0) score_kernel<<<dim3(a.chunks, a.Hkv, a.B), 128, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
@@ -223,15 +518,17 @@ int tt_paged_split(const void* q, const void* k, const void* v, const int* table
                    int chunks, float scale, int dtype, cudaStream_t st) {
   if (B <= 0 || H <= 0) return 0;
   if (Hkv <= 0 || H % Hkv) return -12;
-  if (B > 65535) return -2;
+  if (B > kMaxBatch) return -2;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -4;
   Args a{q, k, v, tables, lens, out, lse, sinks, scores, ws_o, static_cast<float2*>(ws_ml), static_cast<float2*>(ws_tot), ws_x,
          strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8],
          B, H, Hkv, page, width, pages, window, span, chunks, scale};
 #define PICK(T)                                   \
   switch (D) {                                    \
-    case 64: return launch<T, 64>(a, st);         \
-    case 128: return launch<T, 128>(a, st);       \
-    case 256: return launch<T, 256>(a, st);       \
+    case 64: return H / Hkv > kTile ? launch<T, 64, 2>(a, sms, st) : launch<T, 64, 1>(a, sms, st);     \
+    case 128: return H / Hkv > kTile ? launch<T, 128, 2>(a, sms, st) : launch<T, 128, 1>(a, sms, st);  \
+    case 256: return H / Hkv > kTile ? launch<T, 256, 2>(a, sms, st) : launch<T, 256, 1>(a, sms, st);  \
     default: return -10;                          \
   }
   if (dtype == 0) { PICK(__nv_bfloat16) }
