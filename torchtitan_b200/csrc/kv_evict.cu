@@ -4,11 +4,16 @@
 // and, of the n - recent before them, the keep - recent with the largest score, ties going to the lowest index. What stays
 // is copied, in its order, to the first slots of new pages: the old pages are only read, so they may be shared.
 //
-// Selection: the score's bits, mapped so that unsigned order is score order, are cut 8 at a time from the top: a histogram
-// of the digit among the tokens that match the digits found so far gives the next digit of the keep-th largest. Four passes
-// find it exactly; what equals it is taken in index order until the count is full.
+// Selection: the score's bits, mapped so that unsigned order is score order, lie in some range [lo, hi] of keys. A histogram
+// of 2048 equal parts of that range says which part the last kept key is in; that part is the next range, until the range is
+// one key or all of it is kept (at most three rounds of 11 bits each; usually two, since the first splits the occupied part
+// of the scale rather than the 32 bits). Of the keys in the last range the first in index order are taken. A cluster of CTAs
+// shares one (sequence, kv head): each holds its part of the keys in shared memory and reads the others' histograms there.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -19,7 +24,7 @@ struct Args {
   int *new_lens, *kept;      // [B], [B, Hkv, keep]
   long long k_page, k_tok, k_head, v_page, v_tok, v_head;   // bytes
   long long table_row, fresh_row;
-  int B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent;
+  int B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held;   // held: keys of a CTA that fit its shared memory
 };
 
 // Larger key = kept earlier. NaN counts as the largest value, both zeros are one value.
@@ -40,81 +45,155 @@ __device__ __forceinline__ uint32_t key_at(const Args& a, int b, int h, int t) {
   return key_of(a.scores[(static_cast<long long>(p) * a.Hkv + h) * a.page + t % a.page]);
 }
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kMostHeld = 48 * 1024;      // keys
 
-// CTA = (kv head, sequence): writes the kept indices in order.
+// Exclusive sum over the block's threads; total: the sum of all.
+__device__ __forceinline__ int block_scan(int v, int* s_warp, int& total) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += up;
+  }
+  if (lane == 31) s_warp[warp] = inc;
+  __syncthreads();
+  const int mine = s_warp[lane];
+  int w = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += up;
+  }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w - mine, warp);
+  __syncthreads();
+  return before + inc - v;
+}
+
+// Cluster = (kv head, sequence), its CTAs cut the tokens into equal parts: writes the kept indices in order.
 __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int parts = cluster.num_blocks(), part = cluster.block_rank();
+  const int h = blockIdx.x / parts, b = blockIdx.y, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int n = length_of(a, b), left = min(n, a.keep);
   int* kept = a.kept + (static_cast<long long>(b) * a.Hkv + h) * a.keep;
-  if (h == 0 && tid == 0) a.new_lens[b] = left;
-  for (int j = left + tid; j < a.keep; j += kThreads) kept[j] = -1;
-  if (n <= a.keep) {
-    for (int j = tid; j < n; j += kThreads) kept[j] = j;
+  if (blockIdx.x == 0 && tid == 0) a.new_lens[b] = left;
+  for (int j = left + part * kThreads + tid; j < a.keep; j += parts * kThreads) kept[j] = -1;
+  if (n <= a.keep) {                       // the same for the whole cluster
+    for (int j = part * kThreads + tid; j < n; j += parts * kThreads) kept[j] = j;
     return;
   }
   const int old = n - a.recent;
-  int want = a.keep - a.recent;       // of the first `old` tokens
-  __shared__ int hist[256];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_want, s_base, s_ties;
-  __shared__ int s_warp[32], s_warp_t[32];
-  uint32_t prefix = 0;
-  if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
-      __syncthreads();
-      for (int t = tid; t < old; t += kThreads) {
-        const uint32_t key = key_at(a, b, h, t);
-        if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int d = 255, above = 0;
-        while (d > 0 && above + hist[d] < want) above += hist[d--];
-        s_want = want - above;
-        s_prefix = prefix | (static_cast<uint32_t>(d) << shift);
-      }
-      __syncthreads();
-      want = s_want;
-      prefix = s_prefix;
-      __syncthreads();
-    }
-  }
-  // now `want` of the tokens that equal prefix are taken, lowest index first, and all above it
-  if (tid == 0) { s_base = 0; s_ties = 0; }
+  for (int j = part * kThreads + tid; j < a.recent; j += parts * kThreads) kept[a.keep - a.recent + j] = old + j;
+  int want = a.keep - a.recent;            // of the first `old` tokens
+  if (want == 0) return;
+
+  extern __shared__ uint32_t keys[];
+  __shared__ int hist[2][kBins];
+  __shared__ uint32_t s_lo, s_hi;
+  __shared__ int s_warp[kWarps], s_want, s_bin, s_in_bin;
+  __shared__ int s_above, s_equal;
+  const int per = (old + parts - 1) / parts, t0 = min(old, part * per), count = min(old, t0 + per) - t0;
+  auto key = [&](int i) { return i < a.held ? keys[i] : key_at(a, b, h, t0 + i); };
+
+  if (tid == 0) { s_lo = 0xffffffffu; s_hi = 0; }
+  for (int i = tid; i < 2 * kBins; i += kThreads) hist[0][i] = 0;
   __syncthreads();
-  for (int t0 = 0; t0 < n; t0 += kThreads) {
-    const int t = t0 + tid;
-    bool take = false, tie = false;
-    if (t < n) {
-      if (t >= old) take = true;
-      else if (a.keep > a.recent) {
-        const uint32_t key = key_at(a, b, h, t);
-        take = key > prefix;
-        tie = key == prefix;
+  uint32_t lo = 0xffffffffu, hi = 0;
+  for (int i = tid; i < count; i += kThreads) {
+    const uint32_t k = key_at(a, b, h, t0 + i);
+    if (i < a.held) keys[i] = k;
+    lo = min(lo, k);
+    hi = max(hi, k);
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) { atomicMin(&s_lo, lo); atomicMax(&s_hi, hi); }
+  cluster.sync();
+  lo = 0xffffffffu, hi = 0;
+  for (int p = 0; p < parts; ++p) {
+    lo = min(lo, *cluster.map_shared_rank(&s_lo, p));
+    hi = max(hi, *cluster.map_shared_rank(&s_hi, p));
+  }
+  // invariant: `want` of the keys in [lo, hi] are kept, and all above hi
+  for (int round = 0; lo < hi; ++round) {
+    int* mine = hist[round & 1];
+    const int shift = max(0, 21 - __clz(hi - lo));
+    for (int i = tid; i < count; i += kThreads) {
+      const uint32_t k = key(i);
+      if (k >= lo && k <= hi) atomicAdd(&mine[(k - lo) >> shift], 1);
+    }
+    cluster.sync();
+    // bins from the top, two to a thread
+    int c[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      c[e] = 0;
+      for (int p = 0; p < parts; ++p) c[e] += cluster.map_shared_rank(mine, p)[kBins - 1 - 2 * tid - e];
+    }
+    int total;
+    const int before = block_scan(c[0] + c[1], s_warp, total);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int above = before + (e ? c[0] : 0);
+      if (above < want && above + c[e] >= want) {
+        s_bin = kBins - 1 - 2 * tid - e;
+        s_want = want - above;
+        s_in_bin = c[e];
       }
     }
-    const uint32_t tie_mask = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) s_warp_t[warp] = __popc(tie_mask);
+    // the histogram of the round after next; the others are done with the one of the round before this one
+    for (int i = tid; i < kBins; i += kThreads) hist[(round + 1) & 1][i] = 0;
     __syncthreads();
-    int before = s_ties;
-    for (int w = 0; w < warp; ++w) before += s_warp_t[w];
-    if (tie && before + __popc(tie_mask & ((1u << lane) - 1)) < want) take = true;
-    const uint32_t mask = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) s_warp[warp] = __popc(mask);
+    lo += static_cast<uint32_t>(s_bin) << shift;
+    hi = lo + min(hi - lo, (1u << shift) - 1);
+    want = s_want;
+    const bool all = s_in_bin == want;
     __syncthreads();
-    int at = s_base;
-    for (int w = 0; w < warp; ++w) at += s_warp[w];
-    if (take) kept[at + __popc(mask & ((1u << lane) - 1))] = t;
-    __syncthreads();
-    if (tid == 0)
-      for (int w = 0; w < 32; ++w) { s_base += s_warp[w]; s_ties += s_warp_t[w]; }
-    __syncthreads();
+    if (all) break;
   }
+  // kept: above hi, and the first `want` in [lo, hi]. A warp owns a run of consecutive tokens.
+  const int run = (count + kWarps - 1) / kWarps, i0 = min(count, warp * run), i1 = min(count, i0 + run);
+  int above = 0, equal = 0;
+  for (int i = i0 + lane; i < i1; i += 32) {
+    const uint32_t k = key(i);
+    above += k > hi;
+    equal += k >= lo && k <= hi;
+  }
+  above = __reduce_add_sync(0xffffffffu, above);
+  equal = __reduce_add_sync(0xffffffffu, equal);
+  int all_above, all_equal;
+  int above_at = block_scan(lane == 0 ? above : 0, s_warp, all_above);
+  int equal_at = block_scan(lane == 0 ? equal : 0, s_warp, all_equal);
+  if (tid == 0) { s_above = all_above; s_equal = all_equal; }
+  cluster.sync();
+  for (int p = 0; p < part; ++p) {
+    above_at += *cluster.map_shared_rank(&s_above, p);
+    equal_at += *cluster.map_shared_rank(&s_equal, p);
+  }
+  above_at = __shfl_sync(0xffffffffu, above_at, 0);
+  equal_at = __shfl_sync(0xffffffffu, equal_at, 0);
+  const uint32_t below = (1u << lane) - 1;
+  for (int i = i0; i < i1; i += 32) {
+    const bool in = i + lane < i1;
+    const uint32_t k = in ? key(i + lane) : 0;
+    const uint32_t am = __ballot_sync(0xffffffffu, in && k > hi), em = __ballot_sync(0xffffffffu, in && k >= lo && k <= hi);
+    const int rank = equal_at + __popc(em & below);              // among those in [lo, hi]
+    const bool take = ((am >> lane) & 1) || (((em >> lane) & 1) && rank < want);
+    if (take) kept[above_at + __popc(am & below) + min(rank, want)] = t0 + i + lane;
+    above_at += __popc(am);
+    equal_at += __popc(em);
+  }
+  cluster.sync();                          // no CTA leaves while another may read its shared memory
 }
 
-// One thread per 16 bytes of a kept row; the first of a row's threads moves its score too.
+// kRowsEach kept rows to a group of row_bytes / 16 threads, 16 bytes of each row's key and value to a thread, all loads before
+// the stores; the first thread of a group moves the scores.
+constexpr int kRowsEach = 4;
+
 __global__ void __launch_bounds__(256) move_kernel(const Args a) {
   const int per = a.row_bytes / 16;
   const int b = blockIdx.y;
@@ -123,18 +202,33 @@ __global__ void __launch_bounds__(256) move_kernel(const Args a) {
   const int c = static_cast<int>(i % per);
   const long long r = i / per;
   const int h = static_cast<int>(r % a.Hkv);
-  const long long j = r / a.Hkv;
-  if (j >= left) return;
-  const int t = a.kept[(static_cast<long long>(b) * a.Hkv + h) * a.keep + j];
-  const int sp = a.tables[b * a.table_row + t / a.page], dp = a.fresh[b * a.fresh_row + j / a.page];
-  if (sp < 0 || sp >= a.pages || dp < 0 || dp >= a.pages) return;
-  const int so = t % a.page, to = static_cast<int>(j % a.page);
-  *reinterpret_cast<uint4*>(a.k + dp * a.k_page + to * a.k_tok + h * a.k_head + c * 16) =
-      *reinterpret_cast<const uint4*>(a.k + sp * a.k_page + so * a.k_tok + h * a.k_head + c * 16);
-  *reinterpret_cast<uint4*>(a.v + dp * a.v_page + to * a.v_tok + h * a.v_head + c * 16) =
-      *reinterpret_cast<const uint4*>(a.v + sp * a.v_page + so * a.v_tok + h * a.v_head + c * 16);
-  if (c == 0)
-    a.scores[(static_cast<long long>(dp) * a.Hkv + h) * a.page + to] = a.scores[(static_cast<long long>(sp) * a.Hkv + h) * a.page + so];
+  const long long j0 = r / a.Hkv * kRowsEach;
+  if (j0 >= left) return;
+  const int* kept = a.kept + (static_cast<long long>(b) * a.Hkv + h) * a.keep;
+  uint4 kv[kRowsEach], vv[kRowsEach];
+  float s[kRowsEach];
+  long long dst_page[kRowsEach];
+#pragma unroll
+  for (int u = 0; u < kRowsEach; ++u) {
+    const int j = static_cast<int>(j0) + u;
+    dst_page[u] = -1;
+    if (j >= left) continue;
+    const int t = kept[j];
+    const int sp = a.tables[b * a.table_row + t / a.page], dp = a.fresh[b * a.fresh_row + j / a.page], so = t % a.page;
+    if (sp < 0 || sp >= a.pages || dp < 0 || dp >= a.pages) continue;
+    dst_page[u] = dp;
+    kv[u] = *reinterpret_cast<const uint4*>(a.k + sp * a.k_page + so * a.k_tok + h * a.k_head + c * 16);
+    vv[u] = *reinterpret_cast<const uint4*>(a.v + sp * a.v_page + so * a.v_tok + h * a.v_head + c * 16);
+    if (c == 0) s[u] = a.scores[(static_cast<long long>(sp) * a.Hkv + h) * a.page + so];
+  }
+#pragma unroll
+  for (int u = 0; u < kRowsEach; ++u) {
+    if (dst_page[u] < 0) continue;
+    const int to = static_cast<int>((j0 + u) % a.page);
+    *reinterpret_cast<uint4*>(a.k + dst_page[u] * a.k_page + to * a.k_tok + h * a.k_head + c * 16) = kv[u];
+    *reinterpret_cast<uint4*>(a.v + dst_page[u] * a.v_page + to * a.v_tok + h * a.v_head + c * 16) = vv[u];
+    if (c == 0) a.scores[(dst_page[u] * a.Hkv + h) * a.page + to] = s[u];
+  }
 }
 
 }  // namespace
@@ -149,11 +243,28 @@ int tt_kv_evict(void* k, void* v, float* scores, const int* tables, const int* l
   if (B > 65535 || row_bytes % 16 || keep < 1 || recent < 0 || recent > keep) return -2;
   const long long room = static_cast<long long>(width) * page, most = room < keep ? room : keep;
   if (most > static_cast<long long>(fresh_width) * page) return -2;
+  // CTAs of a (sequence, kv head): as many as give every SM one, but none with fewer than 2048 tokens
+  int parts = 1;
+  while (parts < 8 && static_cast<long long>(B) * Hkv * parts < 148 && room / (2 * parts) >= 2048) parts *= 2;
+  const long long per = (room + parts - 1) / parts;
+  const int held = static_cast<int>(per < kMostHeld ? per : kMostHeld);
   Args a{static_cast<char*>(k), static_cast<char*>(v), scores, tables, lens, fresh, new_lens, kept,
          strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7],
-         B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent};
-  select_kernel<<<dim3(Hkv, B), kThreads, 0, st>>>(a);
-  const long long threads = most * Hkv * (row_bytes / 16);
+         B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held};
+  if (cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostHeld * 4) != cudaSuccess) return -4;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(Hkv * parts, B);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(held) * 4;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, select_kernel, a) != cudaSuccess) return -4;
+  const long long threads = (most + kRowsEach - 1) / kRowsEach * Hkv * (row_bytes / 16);
   if (threads > 0) move_kernel<<<dim3(static_cast<unsigned>((threads + 255) / 256), B), 256, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
