@@ -21,10 +21,10 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kMinChunk = 256;    // tokens
+constexpr int kMinChunk = 512;    // tokens
 constexpr int kMaxChunks = 128;   // per sequence: bounds the workspace and the join's work
 constexpr int kTile = 8;          // query heads of one kv head in a tile of columns
-constexpr int kMaxBatch = 4096;   // sequences of one launch (their chunk counts are kept in shared memory)
+constexpr int kMaxBatch = 2048;   // sequences of one launch (their chunk counts are kept in shared memory)
 
 struct Args {
   const void *q, *k, *v;
@@ -38,7 +38,8 @@ struct Args {
   float2* ws_tot;      // [B, H]: M and the denominator (with scores)
   float* ws_x;         // [B, Hkv, span, H / Hkv] (with scores)
   long long q_b, q_h, k_page, k_tok, k_head, v_page, v_tok, v_head, table_row;
-  int B, H, Hkv, page, width, pages, window, span, chunks;
+  int B, H, Hkv, page, width, pages, window, span, chunks, page_shift;
+  bool whole;                                   // a step's tokens lie on one page
   float scale;
 };
 
@@ -62,43 +63,26 @@ __device__ __forceinline__ Range range_of(const Args& a, int b) {
   return r;
 }
 
-template <typename T> __device__ __forceinline__ float to_f(T v);
-template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T from_f(float v);
-template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16(v); }
-template <> __device__ __forceinline__ __half from_f(float v) { return __float2half(v); }
-
 __device__ __forceinline__ int page_of(const Args& a, int b, int t) {
   const int p = a.tables[b * a.table_row + t / a.page];
   return p >= 0 && p < a.pages ? p : -1;
 }
 
-// The end of a query head: sink, division, output. top, sum, x: maximum, sum and weighted values over all of its tokens.
-template <typename T, int D>
-__device__ __forceinline__ void finish(const Args& a, int b, int h, int d, float top, float sum, float x) {
-  const long long bh = static_cast<long long>(b) * a.H + h;
-  if (a.sinks) {
-    const float sink = a.sinks[h] * kLog2e, all = fmaxf(top, sink), base = all == -INFINITY ? 0.f : all;
-    const float f = exp2f(top - base);
-    x *= f;
-    sum = sum * f + exp2f(sink - base);
-    top = all;
-  }
-  static_cast<T*>(a.out)[bh * D + d] = from_f<T>(sum == 0.f ? 0.f : x / sum);
-  if (d == 0) {
-    if (a.lse) a.lse[bh] = (top + log2f(sum)) * kLn2;
-    if (a.ws_tot) a.ws_tot[bh] = make_float2(top, sum);
-  }
-}
-
 // ---- pieces of the matrix path
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {   // zeros where !ok (src is not read then)
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void wait_group() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float ex2(float x) {      // 2^x, off by at most 2^-22 of it; results below 2^-126 are 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
@@ -133,13 +117,36 @@ template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v);
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 
+// The end of a query head: sink, division, output of dims d and d + 1. top, sum, x: maximum, sum and weighted values over all
+// of its tokens.
+template <typename T, int D>
+__device__ __forceinline__ void finish(const Args& a, int b, int h, int d, float top, float sum, float2 x) {
+  const long long bh = static_cast<long long>(b) * a.H + h;
+  if (a.sinks) {
+    const float sink = a.sinks[h] * kLog2e, all = fmaxf(top, sink), base = all == -INFINITY ? 0.f : all;
+    const float f = exp2f(top - base);
+    x.x *= f;
+    x.y *= f;
+    sum = sum * f + exp2f(sink - base);
+    top = all;
+  }
+  *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + bh * D + d) = sum == 0.f ? 0u : pack2<T>(x.x / sum, x.y / sum);
+  if (d == 0) {
+    if (a.lse) a.lse[bh] = (top + log2f(sum)) * kLn2;
+    if (a.ws_tot) a.ws_tot[bh] = make_float2(top, sum);
+  }
+}
+
 constexpr int kWarps = 4;
 constexpr int kRows = 16;        // tokens of one step of a warp
 
-constexpr int kPitch = 64 + 4;   // merged values are passed on 64 dims at a time, rows 4 banks apart
+constexpr int kMerge = 32;        // dims of the warps' results that are merged at a time
+constexpr int kPitch = kMerge + 4;
 
+// A stage: kRows rows of K, then of V. Rows lie 16 bytes more than their length apart, so that the eight rows of a matrix
+// load touch different banks.
 template <int D> struct Ring {
-  static constexpr int kRowBytes = 2 * D, kStageBytes = 2 * kRows * kRowBytes;     // K rows, then V rows
+  static constexpr int kRowBytes = 2 * D, kRowPitch = kRowBytes + 16, kStageBytes = 2 * kRows * kRowPitch;
   static constexpr int kStages = D == 64 ? 6 : 3;
   static constexpr int kBytes = kWarps * kStages * kStageBytes;
 };
@@ -147,28 +154,31 @@ template <int D, int NT> constexpr int smem_bytes() {
   return Ring<D>::kBytes + kWarps * kTile * kPitch * 4 + kWarps * kTile * NT * 8 + (D == 256 ? NT * (D / 16) * 32 * 8 : 0);
 }
 
-// One piece of work: chunk c of sequence b for head tile hkt (kv head x tile of NT * 8 query heads).
+// One piece of work: chunk c of sequence b for a tile of NT * 8 query heads of kv head hk.
 struct Item {
-  int b, c, hkt, t0, t1, chunks;
+  int b, c, hk, tile, t0, t1, chunks;
   Range r;
 };
 
-// items are numbered ((sequence, chunk), head tile), head tile fastest: neighbours read the same tokens' heads, which lie
+// items are numbered ((sequence, chunk), kv head, tile), the last fastest: neighbours read the same tokens' heads, which lie
 // next to each other in the cache.
-__device__ __forceinline__ void item_at(Item& it, const Args& a, const int* first_chunk, int hkts, int i) {
-  const int bc = i / hkts;
-  it.hkt = i - bc * hkts;
-  int lo = 0, hi = a.B - 1;                       // the last sequence that begins at or before bc
+__device__ __forceinline__ void item_at(Item& it, const Args& a, const int* before, const uint8_t* counts, int hkts, int tiles, int i) {
+  const int bc = i / hkts, hkt = i - bc * hkts;
+  it.hk = hkt / tiles;
+  it.tile = hkt - it.hk * tiles;
+  int lo = 0, hi = (a.B - 1) / 16;                // the last 16 sequences that begin at or before bc
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (first_chunk[mid] <= bc) lo = mid; else hi = mid - 1;
+    if (before[mid] <= bc) lo = mid; else hi = mid - 1;
   }
-  it.b = lo;
-  it.c = bc - first_chunk[lo];
-  it.chunks = first_chunk[lo + 1] - first_chunk[lo];
-  it.r = range_of(a, lo);
+  int c = bc - before[lo], b = lo * 16;
+  while (c >= counts[b]) c -= counts[b++];
+  it.b = b;
+  it.c = c;
+  it.chunks = counts[b];
+  it.r = range_of(a, b);
   const int len = chunk_len(it.r.n - it.r.lo);
-  it.t0 = it.r.lo + it.c * len;
+  it.t0 = it.r.lo + c * len;
   it.t1 = min(it.r.n, it.t0 + len);
 }
 
@@ -179,26 +189,30 @@ __device__ __forceinline__ void item_at(Item& it, const Args& a, const int* firs
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
   using R = Ring<D>;
-  constexpr int CH = D / 8;                       // 16-byte pieces of a row
   constexpr bool QS = D == 256;                   // q's fragments in shared memory: they do not fit the registers
   extern __shared__ __align__(128) unsigned char smem[];
   float* s_o = reinterpret_cast<float*>(smem + R::kBytes);                                   // [warp][8][kPitch]
   float2* s_ml = reinterpret_cast<float2*>(s_o + kWarps * kTile * kPitch);                  // [warp][NT * 8]
   uint2* s_q = reinterpret_cast<uint2*>(s_ml + kWarps * kTile * NT);                         // [NT][D / 16][32]
-  int* first_chunk = reinterpret_cast<int*>(s_q + (QS ? NT * (D / 16) * 32 : 0));            // [B + 1]
+  int* before = reinterpret_cast<int*>(s_q + (QS ? NT * (D / 16) * 32 : 0));                 // [groups of 16 sequences + 1]
+  uint8_t* counts = reinterpret_cast<uint8_t*>(before + (a.B + 15) / 16 + 1);                // [B]
   __shared__ int s_sum[kWarps];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int G = a.H / a.Hkv, tiles = (G + kTile * NT - 1) / (kTile * NT), hkts = a.Hkv * tiles;
 
-  // prefix sums of the sequences' chunk counts
+  // the sequences' chunk counts, and how many chunks come before each 16 of them
   {
-    const int per = (a.B + 32 * kWarps - 1) / (32 * kWarps), b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+    const int groups = (a.B + 15) / 16, per = (groups + 32 * kWarps - 1) / (32 * kWarps);
+    const int first = min(groups, tid * per), last = min(groups, first + per);
     int sum = 0;
-    for (int b = b0; b < b1; ++b) {
-      const Range r = range_of(a, b);
-      const int n = r.n - r.lo;
-      first_chunk[b] = sum;
-      if (n > 0) sum += (n + chunk_len(n) - 1) / chunk_len(n);
+    for (int g = first; g < last; ++g) {
+      before[g] = sum;
+      for (int b = g * 16; b < min(a.B, g * 16 + 16); ++b) {
+        const Range r = range_of(a, b);
+        const int n = r.n - r.lo, c = n > 0 ? (n + chunk_len(n) - 1) / chunk_len(n) : 0;
+        counts[b] = static_cast<uint8_t>(c);
+        sum += c;
+      }
     }
     int inc = sum;
 #pragma unroll
@@ -208,62 +222,80 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
     }
     if (lane == 31) s_sum[warp] = inc;
     __syncthreads();
-    int before = inc - sum;
-    for (int w = 0; w < warp; ++w) before += s_sum[w];
-    for (int b = b0; b < b1; ++b) first_chunk[b] += before;
-    if (tid == 32 * kWarps - 1) first_chunk[a.B] = before + sum;
+    int add = inc - sum;
+    for (int w = 0; w < warp; ++w) add += s_sum[w];
+    for (int g = first; g < last; ++g) before[g] += add;
+    if (tid == 32 * kWarps - 1) before[groups] = add + sum;
     __syncthreads();
   }
-  const int items = first_chunk[a.B] * hkts;
+  const int items = before[(a.B + 15) / 16] * hkts;
   const uint32_t ring = smem_u32(smem) + warp * R::kStages * R::kStageBytes;
   const T* kc = static_cast<const T*>(a.k);
   const T* vc = static_cast<const T*>(a.v);
 
   // ---- the loads: `head` is the item being loaded, ht its next token, page its table entry for row lane % 16
-  Item head;
+  Item head = {};
   int hi = blockIdx.x, ht = 0, page = -1, slot = 0;
+  const T *k_head = kc, *v_head = vc;             // of the item being loaded
   auto look_up = [&]() {                          // the table entry of the step at ht, ahead of its use
     const int t = ht + (lane & 15);
     const bool live = t >= head.r.first && t < head.t1;
-    const int at = live ? t / a.page : 0;
+    const int at = !live ? 0 : a.page_shift >= 0 ? t >> a.page_shift : t / a.page;
     slot = t - at * a.page;
     page = live ? a.tables[head.b * a.table_row + at] : -1;
     if (live && (page < 0 || page >= a.pages)) page = -2;         // named outside the cache
   };
+  auto enter = [&]() {
+    item_at(head, a, before, counts, hkts, tiles, hi);
+    ht = head.t0 + warp * kRows;
+    k_head = kc + head.hk * a.k_head;
+    v_head = vc + head.hk * a.v_head;
+  };
   auto settle = [&]() {                           // the first step at or after (hi, ht) that this warp has
     while (hi < items && ht >= head.t1) {
       hi += gridDim.x;
-      if (hi < items) {
-        item_at(head, a, first_chunk, hkts, hi);
-        ht = head.t0 + warp * kRows;
-      }
+      if (hi < items) enter();
     }
     if (hi < items) look_up();
   };
   if (hi < items) {
-    item_at(head, a, first_chunk, hkts, hi);
-    ht = head.t0 + warp * kRows;
+    enter();
     settle();
   }
-  auto load = [&](int stage) {                    // one commit group, empty when nothing is left
+  // A lane copies 16 bytes of every (256 / D)-th row, of keys and of values; one commit group, empty when nothing is left.
+  constexpr int CH = D / 8, RPI = 32 / CH;        // 16-byte pieces of a row, rows of one copy instruction
+  const int ch = lane % CH, row0 = lane / CH;
+  auto load = [&](int stage) {
     if (hi < items) {
-      const uint32_t dst = ring + stage * R::kStageBytes;
-      const int hk = head.hkt / tiles;
+      uint32_t dst = ring + stage * R::kStageBytes + row0 * R::kRowPitch + ch * 16;
+      if (a.whole && ht >= head.r.first && ht + kRows <= head.t1 && __shfl_sync(0xffffffffu, page, 0) >= 0) {
+        // all sixteen tokens live, and on one page (its size is a multiple of 16, and so is ht)
+        const int p = __shfl_sync(0xffffffffu, page, 0), s = __shfl_sync(0xffffffffu, slot, 0) + row0;
+        const T* ks = k_head + p * a.k_page + s * a.k_tok + ch * 8;
+        const T* vs = v_head + p * a.v_page + s * a.v_tok + ch * 8;
 #pragma unroll
-      for (int i = 0; i < CH / 2; ++i) {
-        const int idx = i * 32 + lane, row = idx / CH, ch = idx % CH;
-        const int p = __shfl_sync(0xffffffffu, page, row), s = __shfl_sync(0xffffffffu, slot, row);
-        const bool ok = p >= 0;
-        const uint32_t at = row * R::kRowBytes + ((ch ^ (row & 7)) << 4);
-        const T* ks = ok ? kc + p * a.k_page + s * a.k_tok + hk * a.k_head + ch * 8 : kc;
-        const T* vs = ok ? vc + p * a.v_page + s * a.v_tok + hk * a.v_head + ch * 8 : vc;
-        if (p == -2) {
-          // a bad page number: a key of NaNs, which makes the whole sequence NaN
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + at), "r"(0x7fff7fffu) : "memory");
-        } else {
-          copy16(dst + at, ks, ok);
+        for (int i = 0; i < kRows / RPI; ++i) {
+          copy16(dst + i * RPI * R::kRowPitch, ks);
+          copy16(dst + kRows * R::kRowPitch + i * RPI * R::kRowPitch, vs);
+          ks += RPI * a.k_tok;
+          vs += RPI * a.v_tok;
         }
-        copy16(dst + kRows * R::kRowBytes + at, vs, ok);
+      } else {
+        // row by row: zeros for masked tokens, whatever the cache holds there, and for the key of a token on a bad page NaN,
+        // which makes the sequence NaN
+#pragma unroll 1
+        for (int i = 0; i < kRows / RPI; ++i) {
+          const int p = __shfl_sync(0xffffffffu, page, i * RPI + row0), s = __shfl_sync(0xffffffffu, slot, i * RPI + row0);
+          const bool ok = p >= 0;
+          const T* ks = ok ? k_head + p * a.k_page + s * a.k_tok + ch * 8 : kc;
+          const T* vs = ok ? v_head + p * a.v_page + s * a.v_tok + ch * 8 : vc;
+          if (p == -2)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0x7fff7fffu) : "memory");
+          else
+            copy16(dst, ks, ok);
+          copy16(dst + kRows * R::kRowPitch, vs, ok);
+          dst += RPI * R::kRowPitch;
+        }
       }
       ht += kWarps * kRows;
       settle();
@@ -278,8 +310,8 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
   const int cx = 2 * (lane & 3);                  // this thread's columns (heads): cx, cx + 1 of each tile
   Item it;
   for (int i = blockIdx.x; i < items; i += gridDim.x) {
-    item_at(it, a, first_chunk, hkts, i);
-    const int hk = it.hkt / tiles, g0 = (it.hkt % tiles) * kTile * NT, ng = min(kTile * NT, G - g0);
+    item_at(it, a, before, counts, hkts, tiles, i);
+    const int hk = it.hk, g0 = it.tile * kTile * NT, ng = min(kTile * NT, G - g0);
     // q as the right operand: column = head, consecutive k in a register
     uint2 qf[QS ? 1 : NT][QS ? 1 : D / 16];
     auto q_frag = [&](int nt, int kk) {
@@ -316,21 +348,23 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
       load(stage == 0 ? R::kStages - 1 : stage - 1);
       wait_group<R::kStages - 1>();
       __syncwarp();
-      const uint32_t ks = ring + stage * R::kStageBytes, vs = ks + kRows * R::kRowBytes;
-      float s[NT][4];
+      const uint32_t ks = ring + stage * R::kStageBytes, vs = ks + kRows * R::kRowPitch;
+      float s[NT][4], s2[NT][4];                  // two chains: a product waits for the one before it
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.f;
       {
-        const int row = lane & 15, half = lane >> 4;
+        const uint32_t at = ks + (lane & 15) * R::kRowPitch + (lane >> 4) * 16;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           uint32_t kf[4];
-          ldm4(kf, ks + row * R::kRowBytes + (((kk * 2 + half) ^ (row & 7)) << 4));
+          ldm4(kf, at + kk * 32);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             uint2 qv;
             if constexpr (QS) qv = s_q[(nt * (D / 16) + kk) * 32 + lane]; else qv = qf[nt][kk];
-            mma<T>(s[nt], kf, qv.x, qv.y);
+            mma<T>(kk & 1 ? s2[nt] : s[nt], kf, qv.x, qv.y);
           }
         }
       }
@@ -340,7 +374,7 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = (e < 2 ? la : lb) ? s[nt][e] * c2 : -INFINITY;
+        for (int e = 0; e < 4; ++e) s[nt][e] = (e < 2 ? la : lb) ? (s[nt][e] + s2[nt][e]) * c2 : -INFINITY;
         if (a.ws_x) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -348,6 +382,7 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
             if (g < ng && (e < 2 ? la : lb)) a.ws_x[((static_cast<long long>(it.b) * a.Hkv + hk) * a.span + (tt - it.r.lo)) * G + g0 + g] = s[nt][e];
           }
         }
+        float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float top = fmaxf(s[nt][e], s[nt][e + 2]);
@@ -355,16 +390,18 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
           top = fmaxf(top, m[nt][e]);
-          const float base = top == -INFINITY ? 0.f : top, f = exp2f(m[nt][e] - base);
+          const float base = top == -INFINITY ? 0.f : top;
+          f[e] = ex2(m[nt][e] - base);
           m[nt][e] = top;
-          s[nt][e] = exp2f(s[nt][e] - base);
-          s[nt][e + 2] = exp2f(s[nt][e + 2] - base);
-          l[nt][e] = l[nt][e] * f + s[nt][e] + s[nt][e + 2];
+          s[nt][e] = ex2(s[nt][e] - base);
+          s[nt][e + 2] = ex2(s[nt][e + 2] - base);
+          l[nt][e] = l[nt][e] * f[e] + s[nt][e] + s[nt][e + 2];
+        }
+        if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
-          for (int dd = 0; dd < D / 16; ++dd) {
-            o[nt][dd][e] *= f;
-            o[nt][dd][e + 2] *= f;
-          }
+          for (int dd = 0; dd < D / 16; ++dd)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nt][dd][e] *= f[e & 1];
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -375,11 +412,11 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
         }
       }
       {
-        const int row = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+        const uint32_t at = vs + ((lane & 7) + ((lane >> 4) << 3)) * R::kRowPitch + ((lane >> 3) & 1) * 16;
 #pragma unroll
         for (int dd = 0; dd < D / 16; ++dd) {
           uint32_t vf[4];
-          ldm4t(vf, vs + row * R::kRowBytes + (((dd * 2 + half) ^ (row & 7)) << 4));
+          ldm4t(vf, at + dd * 32);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma<T>(o[nt][dd], vf, hi_p[nt][0], hi_p[nt][1]);
@@ -403,34 +440,40 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
         if (lane < 4) s_ml[warp * kTile * NT + nt * kTile + cx + e] = make_float2(m[nt][e], x);
       }
     const long long row = static_cast<long long>(it.b) * a.chunks * a.H + static_cast<long long>(it.c) * a.H + hk * G + g0;
+    const int g = tid / 16, d = tid % 16 * 2;     // this thread's head of a tile, and its two dims of kMerge
+    __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      const int gg = nt * kTile + g;
+      float top = -INFINITY, sum = 0.f, f[kWarps];
 #pragma unroll
-      for (int part = 0; part < D / 64; ++part) {
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w * kTile * NT + gg].x);
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 y = s_ml[w * kTile * NT + gg];
+        f[w] = ex2(y.x - base);
+        sum += y.y * f[w];            // NaN tokens leave m alone: 0 * NaN carries a sum of NaN on
+      }
+#pragma unroll
+      for (int part = 0; part < D / kMerge; ++part) {
         float* mine = s_o + warp * kTile * kPitch;
 #pragma unroll
-        for (int dd = 0; dd < 4; ++dd)
+        for (int dd = 0; dd < kMerge / 16; ++dd)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mine[(cx + (e & 1)) * kPitch + dd * 16 + lane / 4 + (e >> 1) * 8] = o[nt][part * 4 + dd][e];
+          for (int e = 0; e < 4; ++e) mine[(cx + (e & 1)) * kPitch + dd * 16 + lane / 4 + (e >> 1) * 8] = o[nt][part * (kMerge / 16) + dd][e];
         __syncthreads();
-        for (int j = tid; j < kTile * 64; j += 32 * kWarps) {
-          const int g = j / 64, d = j % 64, gg = nt * kTile + g;
-          if (gg >= ng) break;
-          float top = -INFINITY, sum = 0.f, x = 0.f;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w * kTile * NT + gg].x);
-          const float base = top == -INFINITY ? 0.f : top;
+        if (gg < ng) {
+          float2 x = make_float2(0.f, 0.f);
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) {
-            const float2 y = s_ml[w * kTile * NT + gg];
-            // NaN tokens leave m alone: a warp that saw nothing else has m = -inf and a NaN sum, which 0 * NaN carries on
-            const float f = exp2f(y.x - base);
-            sum += y.y * f;
-            x += s_o[(w * kTile + g) * kPitch + d] * f;
+            const float2 y = *reinterpret_cast<const float2*>(s_o + (w * kTile + g) * kPitch + d);
+            x.x += y.x * f[w];
+            x.y += y.y * f[w];
           }
-          const int at = part * 64 + d;
+          const int at = part * kMerge + d;
           if (it.chunks > 1) {
-            a.ws_o[(row + gg) * D + at] = x;
+            *reinterpret_cast<float2*>(a.ws_o + (row + gg) * D + at) = x;
             if (at == 0) a.ws_ml[row + gg] = make_float2(top, sum);
           } else {
             finish<T, D>(a, it.b, hk * G + g0 + gg, at, top, sum, x);
@@ -442,26 +485,53 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
   }
 }
 
-// CTA = (query head, sequence): the chunks in their order.
+// CTA = (query head, sequence): the chunks, D / 2 threads to a chunk, 512 / D of them side by side; the partial sums of the
+// rows of threads are added in their order.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) join_kernel(const Args a) {
-  const int h = blockIdx.x, b = blockIdx.y;
+__global__ void __launch_bounds__(256) join_kernel(const Args a) {
+  constexpr int W = D / 2, S = 256 / W;
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, d = tid % W * 2, s = tid / W;
   const Range r = range_of(a, b);
   const int span = r.n - r.lo, nc = span > 0 ? (span + chunk_len(span) - 1) / chunk_len(span) : 0;
   if (nc == 1) return;                             // written by the split kernel
+  __shared__ float s_f[kMaxChunks], s_top[8], s_sum[8];
+  __shared__ float2 s_x[S][W];
   const float2* ml = a.ws_ml + static_cast<long long>(b) * a.chunks * a.H + h;
   const float* po = a.ws_o + (static_cast<long long>(b) * a.chunks * a.H + h) * D;
-  float top = -INFINITY, sum = r.bad ? NAN : 0.f;
-  for (int c = 0; c < nc; ++c) top = fmaxf(top, ml[static_cast<long long>(c) * a.H].x);
-  const float base = top == -INFINITY ? 0.f : top;
-  for (int c = 0; c < nc; ++c) {
-    const float2 x = ml[static_cast<long long>(c) * a.H];
-    sum += x.y * exp2f(x.x - base);
+  const float2 mine = tid < nc ? ml[static_cast<long long>(tid) * a.H] : make_float2(-INFINITY, 0.f);
+  float top = mine.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (tid % 32 == 0) s_top[tid / 32] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = fmaxf(top, s_top[w]);
+  const float f = ex2(mine.x - (top == -INFINITY ? 0.f : top));
+  if (tid < nc) s_f[tid] = f;
+  float sum = tid < nc ? mine.y * f : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (tid % 32 == 0) s_sum[tid / 32] = sum;
+  __syncthreads();
+  float2 x = make_float2(0.f, 0.f);
+#pragma unroll 4
+  for (int c = s; c < nc; c += S) {
+    const float2 y = *reinterpret_cast<const float2*>(po + static_cast<long long>(c) * a.H * D + d);
+    x.x += y.x * s_f[c];
+    x.y += y.y * s_f[c];
   }
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float o = 0.f;
-    for (int c = 0; c < nc; ++c) o += po[static_cast<long long>(c) * a.H * D + d] * exp2f(ml[static_cast<long long>(c) * a.H].x - base);
-    finish<T, D>(a, b, h, d, top, sum, o);
+  s_x[s][tid % W] = x;
+  __syncthreads();
+  if (s == 0) {
+    sum = r.bad ? NAN : 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) sum += s_sum[w];
+#pragma unroll
+    for (int i = 1; i < S; ++i) {
+      x.x += s_x[i][tid].x;
+      x.y += s_x[i][tid].y;
+    }
+    finish<T, D>(a, b, h, d, top, sum, x);
   }
 }
 
@@ -486,7 +556,7 @@ template <typename T, int D, int NT>
 int launch(const Args& a, int sms, cudaStream_t st) {
   const int G = a.H / a.Hkv, tiles = (G + kTile * NT - 1) / (kTile * NT);
   if (a.chunks > 0) {
-    const int bytes = smem_bytes<D, NT>() + (a.B + 1) * 4;
+    const int bytes = smem_bytes<D, NT>() + ((a.B + 15) / 16 + 1) * 4 + a.B;
     if (bytes > 227 * 1024) return -2;
     if (cudaFuncSetAttribute(split_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -4;
     const long long most = static_cast<long long>(a.B) * a.chunks * a.Hkv * tiles;
@@ -494,7 +564,7 @@ int launch(const Args& a, int sms, cudaStream_t st) {
     const long long grid = static_cast<long long>(sms) * (per_sm > 0 ? per_sm : 1);
     split_kernel<T, D, NT><<<static_cast<unsigned>(most < grid ? most : grid), 32 * kWarps, bytes, st>>>(a);
   }
-  join_kernel<T, D><<<dim3(a.H, a.B), 128, 0, st>>>(a);
+  join_kernel<T, D><<<dim3(a.H, a.B), 256, 0, st>>>(a);
   if (a.scores && a.chunks > 0) score_kernel<<<dim3(a.chunks, a.Hkv, a.B), 128, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
@@ -523,7 +593,7 @@ int tt_paged_split(const void* q, const void* k, const void* v, const int* table
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -4;
   Args a{q, k, v, tables, lens, out, lse, sinks, scores, ws_o, static_cast<float2*>(ws_ml), static_cast<float2*>(ws_tot), ws_x,
          strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8],
-         B, H, Hkv, page, width, pages, window, span, chunks, scale};
+         B, H, Hkv, page, width, pages, window, span, chunks, page & (page - 1) ? -1 : __builtin_ctz(page), page % kRows == 0, scale};
 #define PICK(T)                                   \
   switch (D) {                                    \
     case 64: return H / Hkv > kTile ? launch<T, 64, 2>(a, sms, st) : launch<T, 64, 1>(a, sms, st);     \

@@ -1023,9 +1023,9 @@ def paged_split(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tenso
     """``serving.paged_attention_split`` on the kernels of csrc/paged_split.cu (arguments checked there)."""
     B, H, D = q.shape
     nb, bs, Hkv, _ = k_cache.shape
-    if B > 4096:       # sequences of one launch
-        parts = [paged_split(q[i : i + 4096], k_cache, v_cache, block_tables[i : i + 4096], context_lens[i : i + 4096], scale, window,
-                             sinks, scores, return_lse) for i in range(0, B, 4096)]
+    if B > 2048:       # sequences of one launch
+        parts = [paged_split(q[i : i + 2048], k_cache, v_cache, block_tables[i : i + 2048], context_lens[i : i + 2048], scale, window,
+                             sinks, scores, return_lse) for i in range(0, B, 2048)]
         return tuple(torch.cat(p) for p in zip(*parts)) if return_lse else torch.cat(parts)
     with torch.cuda.device(q.device):
         if q.stride(2) != 1 or q.data_ptr() % 4 or q.stride(0) % 2 or q.stride(1) % 2:      # read two elements at a time
