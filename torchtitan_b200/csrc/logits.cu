@@ -8,22 +8,20 @@
 // computed in fp32 in this order, each step rounded on its own (no contraction, so that the result does not depend on the
 // compiler), and rounded once to the logits' type. Tokens outside [0, V) in the history and the biases are skipped.
 //
-// The history is a list of tokens. A cluster of CTAs covers the vocabulary (or a slab of it), each CTA one part, for which it
-// keeps a word per token in shared memory: bits 0..19 how often it was generated, bit 20 that it was in the prompt, bits
-// 21..31 one plus its entry in the bias list. The CTAs share the reading of the history and count in the word's owner, so a
-// row's history is read once. Then every CTA streams its part, 16 bytes to a thread.
+// The history is a list of tokens. A CTA takes a part of a row's vocabulary and keeps a word per token of it in shared memory:
+// bits 0..19 how often it was generated, bit 20 that it was in the prompt, bits 21..31 one plus its entry in the bias list.
+// Every CTA of a row reads the whole history for that: it comes from L2, 16 bytes to a thread, and needs no waiting for other
+// CTAs (sharing the reading among a cluster of eight, counting in the owner's shared memory, took longer at every length up
+// to 32768: 24 rows of 50021 logits 34 us against 18, 256 rows of 151936 with 2048 tokens 104 us against 67). Then it
+// streams its part, 16 bytes to a thread, which the L2 has fetched meanwhile.
 #include <cuda_bf16.h>
-#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-namespace cg = cooperative_groups;
-
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kCluster = 8;
 constexpr int kMostPart = 12288;     // logits of one CTA
 constexpr int kMaxBias = 1024;
 constexpr uint32_t kCount = (1u << 20) - 1, kPrompt = 1u << 20;
@@ -61,65 +59,112 @@ __device__ __forceinline__ float adjust(float x, uint32_t w, const Setting& s, c
   return x;
 }
 
-// WORDS: there are penalties or biases (a cluster per slab of the vocabulary); otherwise only the mask is applied.
+// Calls f(token, index) for the row's first n tokens, 16 bytes of them to a thread where they lie on such boundaries.
+template <typename I, typename F>
+__device__ __forceinline__ void each_token(const I* tok, int n, F f) {
+  constexpr int N = 16 / sizeof(I);
+  const int head = min(n, static_cast<int>((16 - reinterpret_cast<uintptr_t>(tok) % 16) % 16 / sizeof(I)));
+  const int vectors = (n - head) / N;
+  for (int i = threadIdx.x; i < head; i += kThreads) f(tok[i], i);
+#pragma unroll 4
+  for (int v = threadIdx.x; v < vectors; v += kThreads) {
+    union { uint4 v; I t[N]; } r;
+    r.v = *reinterpret_cast<const uint4*>(tok + head + v * N);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f(r.t[e], head + v * N + e);
+  }
+  for (int i = head + vectors * N + threadIdx.x; i < n; i += kThreads) f(tok[i], i);
+}
+
+// WORDS: there are penalties or biases; otherwise only the mask is applied.
 template <typename T, bool WORDS>
 __global__ void __launch_bounds__(kThreads) adjust_kernel(const Args a) {
   constexpr int E = 16 / sizeof(T);
   const int b = blockIdx.y, tid = threadIdx.x;
-  const int slab0 = blockIdx.x / kCluster * kCluster * a.part;                  // first logit of the cluster
   const int v0 = min(a.V, static_cast<int>(blockIdx.x) * a.part), v1 = min(a.V, v0 + a.part);
   const T* x = static_cast<const T*>(a.x) + b * a.x_row;
   T* y = static_cast<T*>(a.y) + b * a.y_row;
   // the first logit of the part on a 16-byte boundary of x; word i of the part lies at pad + i, so that the words of a
   // vector lie on such a boundary too
   const int head = static_cast<int>((16 - reinterpret_cast<uintptr_t>(x + v0) % 16) % 16 / sizeof(T)), pad = (E - head) % E;
-  extern __shared__ __align__(16) uint32_t word[];
-  __shared__ __align__(16) int s_id[WORDS ? kMaxBias : 4];
-  __shared__ float s_val[WORDS ? kMaxBias : 1], s_sum[WORDS ? kMaxBias : 1];
+  extern __shared__ __align__(16) uint32_t word[];                       // [part + 2 E]
+  int* s_id = reinterpret_cast<int*>(word + a.part + 2 * E);             // [nb]
+  float* s_val = reinterpret_cast<float*>(s_id + a.nb);                  // [nb]
+  float* s_sum = s_val + a.nb;                                           // [nb]
+  __shared__ uint32_t s_again[WORDS ? kMaxBias / 32 : 1];
+  // the logits come into L2 while the history is counted
+  if (tid == 0 && v1 - v0 >= 2 * E) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(x + v0) & ~uintptr_t{15}, to = reinterpret_cast<uintptr_t>(x + v1) & ~uintptr_t{15};
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(static_cast<uint32_t>(to - from)) : "memory");
+  }
   Setting set{1.f, 0.f, 0.f};
   if constexpr (WORDS) {
-    cg::cluster_group cluster = cg::this_cluster();
     set = {a.rep_t ? a.rep_t[b] : a.rep, a.pres_t ? a.pres_t[b] : a.pres, a.freq_t ? a.freq_t[b] : a.freq};
-    const int nb4 = (a.nb + 3) / 4 * 4;
     for (int i = tid; i < (a.part + 2 * E) / 4; i += kThreads) reinterpret_cast<uint4*>(word)[i] = make_uint4(0, 0, 0, 0);
-    for (int i = tid; i < nb4; i += kThreads) {
-      s_id[i] = i < a.nb ? a.bias_ids[b * a.id_row + i] : -1;
-      s_val[i] = i < a.nb ? a.bias_values[b * a.val_row + i] : 0.f;
+    if (tid < kMaxBias / 32) s_again[tid] = 0;
+    for (int i = tid; i < a.nb; i += kThreads) {
+      s_id[i] = a.bias_ids[b * a.id_row + i];
+      s_val[i] = s_sum[i] = a.bias_values[b * a.val_row + i];
     }
-    cluster.sync();
-    if (a.tokens) {
-      const int n = min(a.L, a.lens ? max(a.lens[b], 0) : a.L), np = a.prompts ? a.prompts[b] : 0;
-      const int slab1 = min(static_cast<long long>(a.V), slab0 + static_cast<long long>(kCluster) * a.part);
-      for (int i = cluster.block_rank() * kThreads + tid; i < n; i += kCluster * kThreads) {
-        const long long t = a.tok64 ? static_cast<const long long*>(a.tokens)[b * a.tok_row + i]
-                                    : static_cast<const int*>(a.tokens)[b * a.tok_row + i];
-        if (t < slab0 || t >= slab1) continue;
-        const int owner = static_cast<int>(t - slab0) / a.part, at = static_cast<int>(t - slab0) - owner * a.part;
-        // the owner's padding follows from its part's address
-        const int o_head = static_cast<int>((16 - reinterpret_cast<uintptr_t>(x + slab0 + owner * a.part) % 16) % 16 / sizeof(T));
-        uint32_t* w = cluster.map_shared_rank(word, owner) + (E - o_head) % E + at;
-        if (i < np) atomicOr(w, kPrompt); else atomicAdd(w, 1u);
-      }
-    }
-    // an entry's token in this part: the first entry of a token sums them all, in their order
+    __syncthreads();
+    // the first entry to come claims its token; another one of the same token marks the claiming entry
+    bool again = false;
     for (int i = tid; i < a.nb; i += kThreads) {
       const int id = s_id[i];
       if (id < v0 || id >= v1) continue;
-      float sum = 0.f;
-      bool first = true;
-      for (int j = 0; j < nb4; j += 4) {
-        const int4 q = *reinterpret_cast<const int4*>(s_id + j);
-        if (q.x == id) { first &= j >= i; sum = __fadd_rn(sum, s_val[j]); }
-        if (q.y == id) { first &= j + 1 >= i; sum = __fadd_rn(sum, s_val[j + 1]); }
-        if (q.z == id) { first &= j + 2 >= i; sum = __fadd_rn(sum, s_val[j + 2]); }
-        if (q.w == id) { first &= j + 3 >= i; sum = __fadd_rn(sum, s_val[j + 3]); }
+      uint32_t* w = &word[pad + id - v0];
+      uint32_t old = *w;
+      while (!(old >> 21)) {
+        const uint32_t seen = atomicCAS(w, old, old | (static_cast<uint32_t>(i + 1) << 21));
+        if (seen == old) break;
+        old = seen;
       }
-      if (first) {
-        s_sum[i] = sum;
-        atomicOr(&word[pad + id - v0], static_cast<uint32_t>(i + 1) << 21);
+      if (const uint32_t by = old >> 21) {
+        atomicOr(&s_again[(by - 1) / 32], 1u << ((by - 1) % 32));
+        again = true;
       }
     }
-    cluster.sync();
+    if (a.tokens) {
+      const int n = min(a.L, a.lens ? max(a.lens[b], 0) : a.L), np = a.prompts ? a.prompts[b] : 0;
+      const uint32_t size = v1 - v0;
+      auto count = [&](long long t, int i) {
+        const unsigned long long at = static_cast<unsigned long long>(t - v0);
+        if (at >= size) return;
+        if (i >= np) atomicAdd(&word[pad + at], 1u); else atomicOr(&word[pad + at], kPrompt);
+      };
+      auto count32 = [&](int t, int i) {
+        const uint32_t at = static_cast<uint32_t>(t) - static_cast<uint32_t>(v0);    // below 0 wraps to 2^31 and more
+        if (at >= size) return;
+        if (i >= np) atomicAdd(&word[pad + at], 1u); else atomicOr(&word[pad + at], kPrompt);
+      };
+      if (a.tok64) each_token(static_cast<const long long*>(a.tokens) + b * a.tok_row, n, count);
+      else each_token(static_cast<const int*>(a.tokens) + b * a.tok_row, n, count32);
+    }
+    if (__syncthreads_or(again)) {
+      // some tokens have several entries: a warp per such token sums them in their order
+      const int lane = tid % 32;
+      int turn = 0;
+      for (int g = 0; g < (a.nb + 31) / 32; ++g) {
+        for (uint32_t todo = s_again[g]; todo; todo &= todo - 1) {
+          if (turn++ % (kThreads / 32) != tid / 32) continue;
+          const int i = g * 32 + __ffs(todo) - 1, id = s_id[i];
+          float sum = 0.f;
+          bool any = false;
+          for (int j0 = 0; j0 < a.nb; j0 += 32) {
+            const int j = j0 + lane;
+            const int other = j < a.nb ? s_id[j] : -1;
+            const float v = j < a.nb ? s_val[j] : 0.f;
+            for (uint32_t same = __ballot_sync(0xffffffffu, other == id); same; same &= same - 1) {
+              const float u = __shfl_sync(0xffffffffu, v, __ffs(same) - 1);
+              sum = any ? __fadd_rn(sum, u) : u;
+              any = true;
+            }
+          }
+          if (lane == 0) s_sum[i] = sum;
+        }
+      }
+      __syncthreads();
+    }
   }
   const uint32_t* mask = a.allowed ? reinterpret_cast<const uint32_t*>(a.allowed) + b * a.mask_row : nullptr;
   auto one = [&](int i) {
@@ -132,6 +177,7 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(const Args a) {
   const int w0 = alike ? min(v1, v0 + head) : v1, w1 = w0 + (v1 - w0) / E * E;
   for (int i = v0 + tid; i < w0; i += kThreads) one(i);
   for (int i = w1 + tid; i < v1; i += kThreads) one(i);
+#pragma unroll 2
   for (int i = w0 + tid * E; i < w1; i += kThreads * E) {
     union { uint4 v; T e[E]; } r;
     r.v = *reinterpret_cast<const uint4*>(x + i);
@@ -148,7 +194,8 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(const Args a) {
       }
     }
     if (mask) {
-      const uint32_t m = __funnelshift_r(mask[i / 32], mask[(i + E - 1) / 32], i % 32);
+      uint32_t m = mask[i / 32] >> (i % 32);
+      if (i % 32 > 32 - E) m |= mask[i / 32 + 1] << (32 - i % 32);       // the vector's bits reach into the next word
 #pragma unroll
       for (int e = 0; e < E; ++e)
         if (!((m >> e) & 1u)) r.e[e] = from_f<T>(-INFINITY);
@@ -160,27 +207,20 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(const Args a) {
 template <typename T>
 int launch(Args a, int B, cudaStream_t st) {
   const bool words = a.tokens || a.nb;
-  // parts of equal size: a cluster (or several) per row, each CTA at most kMostPart logits and, where rows are few, as many
-  // clusters as give every SM a CTA, down to 1024 logits each
-  int slabs = (a.V + kCluster * kMostPart - 1) / (kCluster * kMostPart);
-  while (static_cast<long long>(B) * slabs * kCluster < 148 && a.V / (slabs * kCluster) >= 2048) ++slabs;
-  a.part = ((a.V + slabs * kCluster - 1) / (slabs * kCluster) + 31) / 32 * 32;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kCluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(slabs * kCluster, B);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
+  // parts of equal size, at most kMostPart logits and, where rows are few, as many as give every SM a CTA, down to 1024
+  int parts = (a.V + kMostPart - 1) / kMostPart;
+  if (static_cast<long long>(B) * parts < 148) parts = max(parts, min((147 + B) / B, a.V / 1024));
+  a.part = ((a.V + parts - 1) / parts + 31) / 32 * 32;
+  const dim3 grid((a.V + a.part - 1) / a.part, B);
   if (words) {
-    cfg.dynamicSmemBytes = static_cast<size_t>(a.part + 2 * (16 / sizeof(T))) * 4;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaFuncSetAttribute(adjust_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMostPart + 64) * 4) != cudaSuccess) return -4;
-    return cudaLaunchKernelEx(&cfg, adjust_kernel<T, true>, a) == cudaSuccess ? 0 : -4;
+    const int bytes = (a.part + 2 * (16 / static_cast<int>(sizeof(T)))) * 4 + a.nb * 12;
+    if (cudaFuncSetAttribute(adjust_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMostPart + 64) * 4 + kMaxBias * 12) != cudaSuccess)
+      return -4;
+    adjust_kernel<T, true><<<grid, kThreads, bytes, st>>>(a);
+  } else {
+    adjust_kernel<T, false><<<grid, kThreads, 0, st>>>(a);
   }
-  return cudaLaunchKernelEx(&cfg, adjust_kernel<T, false>, a) == cudaSuccess ? 0 : -4;
+  return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
 }  // namespace
