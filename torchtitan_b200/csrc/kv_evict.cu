@@ -24,7 +24,7 @@ struct Args {
   int *new_lens, *kept;      // [B], [B, Hkv, keep]
   long long k_page, k_tok, k_head, v_page, v_tok, v_head;   // bytes
   long long table_row, fresh_row;
-  int B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held;   // held: keys of a CTA that fit its shared memory
+  int B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held, page_shift;   // held: keys of a CTA that fit its shared memory
 };
 
 // Larger key = kept earlier. NaN counts as the largest value, both zeros are one value.
@@ -46,7 +46,10 @@ __device__ __forceinline__ uint32_t key_at(const Args& a, int b, int h, int t) {
 }
 
 constexpr int kThreads = 1024, kWarps = kThreads / 32;
-constexpr int kBins = 2048;
+static_assert(kWarps == 32, "block_scan keeps one warp sum per lane");
+constexpr int kBins = 2048;           // two to a thread
+constexpr int kMostParts = 8;
+constexpr int kAhead = 4;
 constexpr int kMostHeld = 48 * 1024;      // keys
 
 // Exclusive sum over the block's threads; total: the sum of all.
@@ -75,6 +78,7 @@ __device__ __forceinline__ int block_scan(int v, int* s_warp, int& total) {
 
 // Cluster = (kv head, sequence), its CTAs cut the tokens into equal parts: writes the kept indices in order.
 __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
+  asm volatile("griddepcontrol.launch_dependents;");
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), part = cluster.block_rank();
   const int h = blockIdx.x / parts, b = blockIdx.y, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
@@ -92,7 +96,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
   if (want == 0) return;
 
   extern __shared__ uint32_t keys[];
-  __shared__ int hist[2][kBins];
+  __shared__ __align__(8) int hist[2][kBins];
   __shared__ uint32_t s_lo, s_hi;
   __shared__ int s_warp[kWarps], s_want, s_bin, s_in_bin;
   __shared__ int s_above, s_equal;
@@ -103,21 +107,42 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
   for (int i = tid; i < 2 * kBins; i += kThreads) hist[0][i] = 0;
   __syncthreads();
   uint32_t lo = 0xffffffffu, hi = 0;
-  for (int i = tid; i < count; i += kThreads) {
-    const uint32_t k = key_at(a, b, h, t0 + i);
-    if (i < a.held) keys[i] = k;
-    lo = min(lo, k);
-    hi = max(hi, k);
+  for (int i0 = tid; i0 < count; i0 += kAhead * kThreads) {       // several loads on their way at a time, pages first
+    int page[kAhead], slot[kAhead];
+    uint32_t k[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * kThreads, t = t0 + i, at = a.page_shift >= 0 ? t >> a.page_shift : t / a.page;
+      slot[u] = t - at * a.page;
+      page[u] = i < count ? a.tables[b * a.table_row + at] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const bool ok = page[u] >= 0 && page[u] < a.pages;
+      const float s = ok ? a.scores[(static_cast<long long>(page[u]) * a.Hkv + h) * a.page + slot[u]] : 0.f;
+      k[u] = ok ? key_of(s) : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * kThreads;
+      if (i >= count) continue;
+      if (i < a.held) keys[i] = k[u];
+      lo = min(lo, k[u]);
+      hi = max(hi, k[u]);
+    }
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
   if (lane == 0) { atomicMin(&s_lo, lo); atomicMax(&s_hi, hi); }
-  cluster.sync();
+  auto meet = [&]() { if (parts > 1) cluster.sync(); else __syncthreads(); };
+  meet();
   lo = 0xffffffffu, hi = 0;
-  for (int p = 0; p < parts; ++p) {
-    lo = min(lo, *cluster.map_shared_rank(&s_lo, p));
-    hi = max(hi, *cluster.map_shared_rank(&s_hi, p));
-  }
+#pragma unroll
+  for (int p = 0; p < kMostParts; ++p)
+    if (p < parts) {
+      lo = min(lo, *cluster.map_shared_rank(&s_lo, p));
+      hi = max(hi, *cluster.map_shared_rank(&s_hi, p));
+    }
   // invariant: `want` of the keys in [lo, hi] are kept, and all above hi
   for (int round = 0; lo < hi; ++round) {
     int* mine = hist[round & 1];
@@ -126,13 +151,17 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
       const uint32_t k = key(i);
       if (k >= lo && k <= hi) atomicAdd(&mine[(k - lo) >> shift], 1);
     }
-    cluster.sync();
-    // bins from the top, two to a thread
-    int c[2];
+    meet();
+    // bins from the top, two to a thread; all parts' loads at once
+    int c[2] = {0, 0};
+    int2 of[kMostParts];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      c[e] = 0;
-      for (int p = 0; p < parts; ++p) c[e] += cluster.map_shared_rank(mine, p)[kBins - 1 - 2 * tid - e];
+    for (int p = 0; p < kMostParts; ++p)
+      of[p] = p < parts ? *reinterpret_cast<const int2*>(cluster.map_shared_rank(mine, p) + kBins - 2 - 2 * tid) : make_int2(0, 0);
+#pragma unroll
+    for (int p = 0; p < kMostParts; ++p) {
+      c[0] += of[p].y;
+      c[1] += of[p].x;
     }
     int total;
     const int before = block_scan(c[0] + c[1], s_warp, total);
@@ -169,7 +198,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
   int above_at = block_scan(lane == 0 ? above : 0, s_warp, all_above);
   int equal_at = block_scan(lane == 0 ? equal : 0, s_warp, all_equal);
   if (tid == 0) { s_above = all_above; s_equal = all_equal; }
-  cluster.sync();
+  meet();
   for (int p = 0; p < part; ++p) {
     above_at += *cluster.map_shared_rank(&s_above, p);
     equal_at += *cluster.map_shared_rank(&s_equal, p);
@@ -187,7 +216,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
     above_at += __popc(am);
     equal_at += __popc(em);
   }
-  cluster.sync();                          // no CTA leaves while another may read its shared memory
+  if (parts > 1) cluster.sync();           // no CTA leaves while another may read its shared memory
 }
 
 // kRowsEach kept rows to a group of row_bytes / 16 threads, 16 bytes of each row's key and value to a thread, all loads before
@@ -197,6 +226,7 @@ constexpr int kRowsEach = 4;
 __global__ void __launch_bounds__(256) move_kernel(const Args a) {
   const int per = a.row_bytes / 16;
   const int b = blockIdx.y;
+  asm volatile("griddepcontrol.wait;" ::: "memory");          // started early: the selection must be complete
   const int left = min(length_of(a, b), a.keep);
   const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
   const int c = static_cast<int>(i % per);
@@ -245,12 +275,12 @@ int tt_kv_evict(void* k, void* v, float* scores, const int* tables, const int* l
   if (most > static_cast<long long>(fresh_width) * page) return -2;
   // CTAs of a (sequence, kv head): as many as give every SM one, but none with fewer than 2048 tokens
   int parts = 1;
-  while (parts < 8 && static_cast<long long>(B) * Hkv * parts < 148 && room / (2 * parts) >= 2048) parts *= 2;
+  while (parts < kMostParts && static_cast<long long>(B) * Hkv * parts < 148 && room / (2 * parts) >= 2048) parts *= 2;
   const long long per = (room + parts - 1) / parts;
   const int held = static_cast<int>(per < kMostHeld ? per : kMostHeld);
   Args a{static_cast<char*>(k), static_cast<char*>(v), scores, tables, lens, fresh, new_lens, kept,
          strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7],
-         B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held};
+         B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held, page & (page - 1) ? -1 : __builtin_ctz(page)};
   if (cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostHeld * 4) != cudaSuccess) return -4;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -265,7 +295,15 @@ int tt_kv_evict(void* k, void* v, float* scores, const int* tables, const int* l
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, select_kernel, a) != cudaSuccess) return -4;
   const long long threads = (most + kRowsEach - 1) / kRowsEach * Hkv * (row_bytes / 16);
-  if (threads > 0) move_kernel<<<dim3(static_cast<unsigned>((threads + 255) / 256), B), 256, 0, st>>>(a);
+  if (threads > 0) {
+    // the move's CTAs come up while the selection runs and wait there for its end
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>((threads + 255) / 256), B);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    if (cudaLaunchKernelEx(&cfg, move_kernel, a) != cudaSuccess) return -4;
+  }
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 

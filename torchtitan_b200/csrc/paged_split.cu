@@ -63,11 +63,6 @@ __device__ __forceinline__ Range range_of(const Args& a, int b) {
   return r;
 }
 
-__device__ __forceinline__ int page_of(const Args& a, int b, int t) {
-  const int p = a.tables[b * a.table_row + t / a.page];
-  return p >= 0 && p < a.pages ? p : -1;
-}
-
 // ---- pieces of the matrix path
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -199,6 +194,7 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
   __shared__ int s_sum[kWarps];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int G = a.H / a.Hkv, tiles = (G + kTile * NT - 1) / (kTile * NT), hkts = a.Hkv * tiles;
+  asm volatile("griddepcontrol.launch_dependents;");       // the join's CTAs may come up, and wait for this grid's end
 
   // the sequences' chunk counts, and how many chunks come before each 16 of them
   {
@@ -493,6 +489,8 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, d = tid % W * 2, s = tid / W;
   const Range r = range_of(a, b);
   const int span = r.n - r.lo, nc = span > 0 ? (span + chunk_len(span) - 1) / chunk_len(span) : 0;
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (nc == 1) return;                             // written by the split kernel
   __shared__ float s_f[kMaxChunks], s_top[8], s_sum[8];
   __shared__ float2 s_x[S][W];
@@ -537,18 +535,40 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
 
 // CTA = (chunk, kv head, sequence): a token's weights over the query heads of its kv head, added to its score. One addition
 // per page slot and sequence, atomic only because two sequences may share a page.
-__global__ void __launch_bounds__(128) score_kernel(const Args a) {
-  const int c = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, G = a.H / a.Hkv;
+__global__ void __launch_bounds__(256) score_kernel(const Args a) {
+  const int c = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, G = a.H / a.Hkv, tid = threadIdx.x;
   const Range r = range_of(a, b);
   const int len = chunk_len(r.n - r.lo), t0 = r.lo + c * len, t1 = min(r.n, t0 + len);
-  const float2* tot = a.ws_tot + static_cast<long long>(b) * a.H + hk * G;
-  for (int t = t0 + threadIdx.x; t < t1; t += 128) {
-    const int p = page_of(a, b, t);
-    if (t < r.first || p < 0) continue;
-    const float* x = a.ws_x + ((static_cast<long long>(b) * a.Hkv + hk) * a.span + (t - r.lo)) * G;
-    float w = 0.f;
-    for (int g = 0; g < G; ++g) w += x[g] == -INFINITY ? 0.f : exp2f(x[g] - tot[g].x) / tot[g].y;
-    atomicAdd(a.scores + (static_cast<long long>(p) * a.Hkv + hk) * a.page + t % a.page, w);
+  __shared__ float2 s_tot[64];                    // of 64 heads at a time: M and 1 / l, 0 where there is no weight
+  const float* x = a.ws_x + (static_cast<long long>(b) * a.Hkv + hk) * a.span * G;
+  asm volatile("griddepcontrol.wait;" ::: "memory");        // in every CTA: what follows on the stream relies on it
+  if (t0 >= t1) return;
+  for (int g0 = 0; g0 < G; g0 += 64) {
+    const int ng = min(64, G - g0);
+    __syncthreads();
+    if (tid < ng) {
+      const float2 y = a.ws_tot[static_cast<long long>(b) * a.H + hk * G + g0 + tid];
+      s_tot[tid] = make_float2(y.x == -INFINITY ? 0.f : y.x, y.y == 0.f ? 0.f : 1.f / y.y);
+    }
+    __syncthreads();
+    for (int t = t0 + tid; t < t1; t += 256) {
+      const int at = a.page_shift >= 0 ? t >> a.page_shift : t / a.page;
+      const int p = a.tables[b * a.table_row + at];
+      if (t < r.first || p < 0 || p >= a.pages) continue;
+      const float* xt = x + static_cast<long long>(t - r.lo) * G + g0;
+      float w = 0.f;
+      if (G % 4 == 0) {
+#pragma unroll 2
+        for (int g = 0; g < ng; g += 4) {
+          const float4 y = *reinterpret_cast<const float4*>(xt + g);
+          w += ex2(y.x - s_tot[g].x) * s_tot[g].y + ex2(y.y - s_tot[g + 1].x) * s_tot[g + 1].y +
+               ex2(y.z - s_tot[g + 2].x) * s_tot[g + 2].y + ex2(y.w - s_tot[g + 3].x) * s_tot[g + 3].y;
+        }
+      } else {
+        for (int g = 0; g < ng; ++g) w += ex2(xt[g] - s_tot[g].x) * s_tot[g].y;
+      }
+      atomicAdd(a.scores + (static_cast<long long>(p) * a.Hkv + hk) * a.page + (t - at * a.page), w);
+    }
   }
 }
 
@@ -564,8 +584,22 @@ int launch(const Args& a, int sms, cudaStream_t st) {
     const long long grid = static_cast<long long>(sms) * (per_sm > 0 ? per_sm : 1);
     split_kernel<T, D, NT><<<static_cast<unsigned>(most < grid ? most : grid), 32 * kWarps, bytes, st>>>(a);
   }
-  join_kernel<T, D><<<dim3(a.H, a.B), 256, 0, st>>>(a);
-  if (a.scores && a.chunks > 0) score_kernel<<<dim3(a.chunks, a.Hkv, a.B), 128, 0, st>>>(a);
+  // these come up while the kernel before them runs, and wait for its end (griddepcontrol.wait) before they touch its results
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = a.chunks > 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.H, a.B);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, join_kernel<T, D>, a) != cudaSuccess) return -4;
+  if (a.scores && a.chunks > 0) {
+    cfg.gridDim = dim3(a.chunks, a.Hkv, a.B);
+    cfg.blockDim = dim3(256);
+    if (cudaLaunchKernelEx(&cfg, score_kernel, a) != cudaSuccess) return -4;
+  }
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
