@@ -13,6 +13,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace cg = cooperative_groups;
 
 namespace {
@@ -281,7 +283,13 @@ int tt_kv_evict(void* k, void* v, float* scores, const int* tables, const int* l
   Args a{static_cast<char*>(k), static_cast<char*>(v), scores, tables, lens, fresh, new_lens, kept,
          strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7],
          B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held, page & (page - 1) ? -1 : __builtin_ctz(page)};
-  if (cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostHeld * 4) != cudaSuccess) return -4;
+  static std::atomic<uint64_t> ready{0};          // devices on which the kernel may take its shared memory
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -4;
+  if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    if (cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostHeld * 4) != cudaSuccess) return -4;
+    ready.fetch_or(uint64_t{1} << dev);
+  }
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = parts;

@@ -19,6 +19,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace {
 
 constexpr int kThreads = 512;
@@ -214,8 +216,14 @@ int launch(Args a, int B, cudaStream_t st) {
   const dim3 grid((a.V + a.part - 1) / a.part, B);
   if (words) {
     const int bytes = (a.part + 2 * (16 / static_cast<int>(sizeof(T)))) * 4 + a.nb * 12;
-    if (cudaFuncSetAttribute(adjust_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMostPart + 64) * 4 + kMaxBias * 12) != cudaSuccess)
-      return -4;
+    static std::atomic<uint64_t> ready{0};        // devices on which the kernel may take its shared memory
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -4;
+    if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+      if (cudaFuncSetAttribute(adjust_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMostPart + 64) * 4 + kMaxBias * 12) != cudaSuccess)
+        return -4;
+      ready.fetch_or(uint64_t{1} << dev);
+    }
     adjust_kernel<T, true><<<grid, kThreads, bytes, st>>>(a);
   } else {
     adjust_kernel<T, false><<<grid, kThreads, 0, st>>>(a);

@@ -17,6 +17,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -39,7 +41,7 @@ struct Args {
   float* ws_x;         // [B, Hkv, span, H / Hkv] (with scores)
   long long q_b, q_h, k_page, k_tok, k_head, v_page, v_tok, v_head, table_row;
   int B, H, Hkv, page, width, pages, window, span, chunks, page_shift;
-  bool whole;                                   // a step's tokens lie on one page
+  bool whole;                                   // every eight tokens of a step lie on one page
   float scale;
 };
 
@@ -142,7 +144,7 @@ constexpr int kPitch = kMerge + 4;
 // load touch different banks.
 template <int D> struct Ring {
   static constexpr int kRowBytes = 2 * D, kRowPitch = kRowBytes + 16, kStageBytes = 2 * kRows * kRowPitch;
-  static constexpr int kStages = D == 64 ? 6 : 3;
+  static constexpr int kStages = 3;
   static constexpr int kBytes = kWarps * kStages * kStageBytes;
 };
 template <int D, int NT> constexpr int smem_bytes() {
@@ -200,15 +202,17 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
   {
     const int groups = (a.B + 15) / 16, per = (groups + 32 * kWarps - 1) / (32 * kWarps);
     const int first = min(groups, tid * per), last = min(groups, first + per);
+#pragma unroll 4
+    for (int b = tid; b < a.B; b += 32 * kWarps) {
+      const Range r = range_of(a, b);
+      const int n = r.n - r.lo;
+      counts[b] = static_cast<uint8_t>(n > 0 ? (n + chunk_len(n) - 1) / chunk_len(n) : 0);
+    }
+    __syncthreads();
     int sum = 0;
     for (int g = first; g < last; ++g) {
       before[g] = sum;
-      for (int b = g * 16; b < min(a.B, g * 16 + 16); ++b) {
-        const Range r = range_of(a, b);
-        const int n = r.n - r.lo, c = n > 0 ? (n + chunk_len(n) - 1) / chunk_len(n) : 0;
-        counts[b] = static_cast<uint8_t>(c);
-        sum += c;
-      }
+      for (int b = g * 16; b < min(a.B, g * 16 + 16); ++b) sum += counts[b];
     }
     int inc = sum;
 #pragma unroll
@@ -264,22 +268,27 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
   auto load = [&](int stage) {
     if (hi < items) {
       uint32_t dst = ring + stage * R::kStageBytes + row0 * R::kRowPitch + ch * 16;
-      if (a.whole && ht >= head.r.first && ht + kRows <= head.t1 && __shfl_sync(0xffffffffu, page, 0) >= 0) {
-        // all sixteen tokens live, and on one page (its size is a multiple of 16, and so is ht)
-        const int p = __shfl_sync(0xffffffffu, page, 0), s = __shfl_sync(0xffffffffu, slot, 0) + row0;
-        const T* ks = k_head + p * a.k_page + s * a.k_tok + ch * 8;
-        const T* vs = v_head + p * a.v_page + s * a.v_tok + ch * 8;
+      const int pa = __shfl_sync(0xffffffffu, page, 0), pb = __shfl_sync(0xffffffffu, page, 8);
+      if (a.whole && ht >= head.r.first && ht + kRows <= head.t1 && pa >= 0 && pb >= 0) {
+        // all sixteen tokens live, each eight of them on one page (its size is a multiple of 8, and so is ht)
+        const int sa = __shfl_sync(0xffffffffu, slot, 0) + row0, sb = __shfl_sync(0xffffffffu, slot, 8) + row0;
 #pragma unroll
-        for (int i = 0; i < kRows / RPI; ++i) {
-          copy16(dst + i * RPI * R::kRowPitch, ks);
-          copy16(dst + kRows * R::kRowPitch + i * RPI * R::kRowPitch, vs);
-          ks += RPI * a.k_tok;
-          vs += RPI * a.v_tok;
+        for (int h = 0; h < 2; ++h) {
+          const T* ks = k_head + (h ? pb : pa) * a.k_page + (h ? sb : sa) * a.k_tok + ch * 8;
+          const T* vs = v_head + (h ? pb : pa) * a.v_page + (h ? sb : sa) * a.v_tok + ch * 8;
+#pragma unroll
+          for (int i = 0; i < 8 / RPI; ++i) {
+            const uint32_t at = dst + (h * 8 + i * RPI) * R::kRowPitch;
+            copy16(at, ks);
+            copy16(at + kRows * R::kRowPitch, vs);
+            ks += RPI * a.k_tok;
+            vs += RPI * a.v_tok;
+          }
         }
       } else {
         // row by row: zeros for masked tokens, whatever the cache holds there, and for the key of a token on a bad page NaN,
         // which makes the sequence NaN
-#pragma unroll 1
+#pragma unroll 2
         for (int i = 0; i < kRows / RPI; ++i) {
           const int p = __shfl_sync(0xffffffffu, page, i * RPI + row0), s = __shfl_sync(0xffffffffu, slot, i * RPI + row0);
           const bool ok = p >= 0;
@@ -479,6 +488,13 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
       }
     }
   }
+  if (a.chunks <= 1) {                            // no join follows: sequences without tokens are answered here
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      const Range r = range_of(a, b);
+      if (r.n > 0) continue;
+      for (int j = tid * 2; j < a.H * D; j += 64 * kWarps) finish<T, D>(a, b, j / D, j % D, -INFINITY, r.bad ? NAN : 0.f, make_float2(0.f, 0.f));
+    }
+  }
 }
 
 // CTA = (query head, sequence): the chunks, D / 2 threads to a chunk, 512 / D of them side by side; the partial sums of the
@@ -572,29 +588,44 @@ __global__ void __launch_bounds__(256) score_kernel(const Args a) {
   }
 }
 
-template <typename T, int D, int NT>
-int launch(const Args& a, int sms, cudaStream_t st) {
-  const int G = a.H / a.Hkv, tiles = (G + kTile * NT - 1) / (kTile * NT);
-  if (a.chunks > 0) {
-    const int bytes = smem_bytes<D, NT>() + ((a.B + 15) / 16 + 1) * 4 + a.B;
-    if (bytes > 227 * 1024) return -2;
-    if (cudaFuncSetAttribute(split_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -4;
-    const long long most = static_cast<long long>(a.B) * a.chunks * a.Hkv * tiles;
-    const int per_sm = 228 * 1024 / (bytes + 1024);
-    const long long grid = static_cast<long long>(sms) * (per_sm > 0 ? per_sm : 1);
-    split_kernel<T, D, NT><<<static_cast<unsigned>(most < grid ? most : grid), 32 * kWarps, bytes, st>>>(a);
+constexpr int kMostSmem = 227 * 1024 - 1024;       // dynamic; the rest is for the static variables
+
+int sm_count(int dev) {
+  static std::atomic<int> known[64];
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (!n) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n = 148;
+    known[dev].store(n, std::memory_order_relaxed);
   }
+  return n;
+}
+
+template <typename T, int D, int NT>
+int launch(const Args& a, int dev, cudaStream_t st) {
+  const int G = a.H / a.Hkv, tiles = (G + kTile * NT - 1) / (kTile * NT);
+  const int bytes = smem_bytes<D, NT>() + ((a.B + 15) / 16 + 1) * 4 + a.B;
+  if (bytes > kMostSmem) return -2;
+  static std::atomic<uint64_t> ready{0};        // devices on which the kernel may take its shared memory
+  if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    if (cudaFuncSetAttribute(split_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem) != cudaSuccess) return -4;
+    ready.fetch_or(uint64_t{1} << dev);
+  }
+  const long long most = static_cast<long long>(a.B) * a.chunks * a.Hkv * tiles;
+  const int per_sm = 228 * 1024 / (bytes + 1024);
+  const long long grid = static_cast<long long>(sm_count(dev)) * (per_sm > 0 ? per_sm : 1);
+  split_kernel<T, D, NT><<<static_cast<unsigned>(most < 1 ? 1 : most < grid ? most : grid), 32 * kWarps, bytes, st>>>(a);
+  if (a.chunks <= 1 && !a.scores) return cudaGetLastError() == cudaSuccess ? 0 : -4;
   // these come up while the kernel before them runs, and wait for its end (griddepcontrol.wait) before they touch its results
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = a.chunks > 0;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.H, a.B);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, join_kernel<T, D>, a) != cudaSuccess) return -4;
+  if (a.chunks > 1 && cudaLaunchKernelEx(&cfg, join_kernel<T, D>, a) != cudaSuccess) return -4;
   if (a.scores && a.chunks > 0) {
     cfg.gridDim = dim3(a.chunks, a.Hkv, a.B);
     cfg.blockDim = dim3(256);
@@ -623,16 +654,16 @@ int tt_paged_split(const void* q, const void* k, const void* v, const int* table
   if (B <= 0 || H <= 0) return 0;
   if (Hkv <= 0 || H % Hkv) return -12;
   if (B > kMaxBatch) return -2;
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -4;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -4;
   Args a{q, k, v, tables, lens, out, lse, sinks, scores, ws_o, static_cast<float2*>(ws_ml), static_cast<float2*>(ws_tot), ws_x,
          strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8],
-         B, H, Hkv, page, width, pages, window, span, chunks, page & (page - 1) ? -1 : __builtin_ctz(page), page % kRows == 0, scale};
+         B, H, Hkv, page, width, pages, window, span, chunks, page & (page - 1) ? -1 : __builtin_ctz(page), page % 8 == 0, scale};
 #define PICK(T)                                   \
   switch (D) {                                    \
-    case 64: return H / Hkv > kTile ? launch<T, 64, 2>(a, sms, st) : launch<T, 64, 1>(a, sms, st);     \
-    case 128: return H / Hkv > kTile ? launch<T, 128, 2>(a, sms, st) : launch<T, 128, 1>(a, sms, st);  \
-    case 256: return H / Hkv > kTile ? launch<T, 256, 2>(a, sms, st) : launch<T, 256, 1>(a, sms, st);  \
+    case 64: return H / Hkv > kTile ? launch<T, 64, 2>(a, dev, st) : launch<T, 64, 1>(a, dev, st);     \
+    case 128: return H / Hkv > kTile ? launch<T, 128, 2>(a, dev, st) : launch<T, 128, 1>(a, dev, st);  \
+    case 256: return H / Hkv > kTile ? launch<T, 256, 2>(a, dev, st) : launch<T, 256, 1>(a, dev, st);  \
     default: return -10;                          \
   }
   if (dtype == 0) { PICK(__nv_bfloat16) }

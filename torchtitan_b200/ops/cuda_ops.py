@@ -12,7 +12,6 @@ so once in the log.
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 
 import torch
@@ -998,6 +997,16 @@ def paged_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tens
 
 
 PAGED_SPLIT_DIMS = (64, 128, 256)
+_PAGED_SPLIT_BATCH = 2048      # sequences of one launch
+
+
+def _elsewhere(device: torch.device) -> bool:
+    """Whether another device than the tensors' is current (the calls below enter it then; a guard costs several us)."""
+    return device.index != torch.cuda.current_device()
+
+
+def _stream_of(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _i32(t: Tensor) -> Tensor:
@@ -1009,97 +1018,128 @@ def _rows_i32(t: Tensor) -> Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _cache_strides(name: str, t: Tensor, unit: int) -> list:
+def _cache_strides(name: str, t: Tensor, size: int, unit: int) -> tuple:
     """(page, token, head) strides in units of ``unit`` bytes of a cache whose heads are contiguous on 16-byte boundaries."""
-    size = t.element_size()
-    strides = [t.stride(i) * size if t.shape[i] > 1 else 0 for i in range(3)]
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 16 for s in strides):
+    page, tok, head, one = t.stride()
+    if 1 in t.shape:        # what is not stepped over may have any stride
+        page, tok, head = (s if n > 1 else 0 for s, n in zip((page, tok, head), t.shape))
+    if one != 1 or (t.data_ptr() | page * size | tok * size | head * size) % 16:
         raise ValueError(f"{name} cache: heads must be contiguous and start on 16-byte boundaries (strides {t.stride()})")
-    return [s // unit for s in strides]
+    return page * size // unit, tok * size // unit, head * size // unit
 
 
 def paged_split(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tensor, context_lens: Tensor, scale: float, window, sinks,
                 scores, return_lse: bool):
     """``serving.paged_attention_split`` on the kernels of csrc/paged_split.cu (arguments checked there)."""
     B, H, D = q.shape
-    nb, bs, Hkv, _ = k_cache.shape
-    if B > 2048:       # sequences of one launch
-        parts = [paged_split(q[i : i + 2048], k_cache, v_cache, block_tables[i : i + 2048], context_lens[i : i + 2048], scale, window,
-                             sinks, scores, return_lse) for i in range(0, B, 2048)]
+    dev = q.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return paged_split(q, k_cache, v_cache, block_tables, context_lens, scale, window, sinks, scores, return_lse)
+    if B > _PAGED_SPLIT_BATCH:
+        parts = [paged_split(*(t[i : i + _PAGED_SPLIT_BATCH] if t is not k_cache and t is not v_cache else t
+                               for t in (q, k_cache, v_cache, block_tables, context_lens)), scale, window, sinks, scores, return_lse)
+                 for i in range(0, B, _PAGED_SPLIT_BATCH)]
         return tuple(torch.cat(p) for p in zip(*parts)) if return_lse else torch.cat(parts)
-    with torch.cuda.device(q.device):
-        if q.stride(2) != 1 or q.data_ptr() % 4 or q.stride(0) % 2 or q.stride(1) % 2:      # read two elements at a time
-            q = q.clone(memory_format=torch.contiguous_format)
-        size = k_cache.element_size()
-        bt, cl = _rows_i32(block_tables), _i32(context_lens).contiguous()
-        if sinks is not None:
-            sinks = sinks.to(torch.float32).contiguous()
-        L = _lib()
-        room = bt.shape[1] * bs
-        win = 0 if window is None else min(int(window), room)
-        if win >= room:
-            win = 0
-        span = min(room, win + 15) if win else room
-        chunks = L.tt_paged_split_chunks(room, win)
-        new = functools.partial(torch.empty, dtype=torch.float32, device=q.device)
-        out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
-        lse = new((B, H)) if return_lse else None
-        ws_o, ws_ml = new((B, chunks, H, D)), new((B, chunks, H, 2))
-        ws_tot, ws_x = (new((B, H, 2)), new((B, H, span))) if scores is not None else (None, None)
-        strides = (ctypes.c_longlong * 9)(q.stride(0), q.stride(1), *_cache_strides("key", k_cache, size),
-                                          *_cache_strides("value", v_cache, size), bt.stride(0))
-        _ck(L.tt_paged_split(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), bt.data_ptr(), cl.data_ptr(), out.data_ptr(),
-                             _p(lse), _p(sinks), _p(scores), ws_o.data_ptr(), ws_ml.data_ptr(), _p(ws_tot), _p(ws_x), strides,
-                             B, H, Hkv, D, bs, bt.shape[1], nb, win, span, chunks, float(scale),
-                             0 if q.dtype == torch.bfloat16 else 2, _stream()), "tt_paged_split")
+    nb, bs, Hkv, _ = k_cache.shape
+    q_b, q_h, q_d = q.stride()
+    if q_d != 1 or (q.data_ptr() | 2 * q_b | 2 * q_h) % 4:      # read two elements at a time
+        q = q.clone(memory_format=torch.contiguous_format)
+        q_b, q_h, _ = q.stride()
+    bt, cl = _rows_i32(block_tables), _i32(context_lens).contiguous()
+    if sinks is not None:
+        sinks = sinks.to(torch.float32).contiguous()
+    L = _lib()
+    width = bt.shape[1]
+    room = width * bs
+    win = 0 if window is None or window >= room else int(window)
+    span = min(room, win + 15) if win else room
+    chunks = L.tt_paged_split_chunks(room, win)
+    out = q.new_empty((B, H, D))
+    lse = torch.empty((B, H), dtype=torch.float32, device=dev) if return_lse else None
+    o = x = ml = tot = None
+    if chunks > 1 or scores is not None:
+        # one allocation: partial outputs, every logit, the partial (maximum, sum) and the joint ones
+        rows = B * H
+        n_o, n_ml = (rows * chunks * D, 2 * rows * chunks) if chunks > 1 else (0, 0)
+        n_x = rows * span + rows * span % 2 if scores is not None else 0         # pairs follow: an even number
+        ws = torch.empty(n_o + n_x + n_ml + (2 * rows if n_x else 0), dtype=torch.float32, device=dev)
+        o = ws.data_ptr()
+        x = o + 4 * n_o
+        ml = x + 4 * n_x
+        tot = ml + 4 * n_ml
+        if not n_x:
+            x = tot = None
+    strides = (ctypes.c_longlong * 9)(q_b, q_h, *_cache_strides("key", k_cache, 2, 2), *_cache_strides("value", v_cache, 2, 2),
+                                      bt.stride(0))
+    _ck(L.tt_paged_split(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), bt.data_ptr(), cl.data_ptr(), out.data_ptr(),
+                         _p(lse), _p(sinks), _p(scores), o, ml, tot, x, strides,
+                         B, H, Hkv, D, bs, width, nb, win, span, chunks, scale, 0 if q.dtype == torch.bfloat16 else 2,
+                         _stream_of(dev)), "tt_paged_split")
     return (out, lse) if return_lse else out
 
 
 def kv_evict(k_cache: Tensor, v_cache: Tensor, scores: Tensor, block_tables: Tensor, context_lens: Tensor, new_tables: Tensor,
              keep: int, recent: int):
     """``serving.kv_cache_evict`` on the kernels of csrc/kv_evict.cu (arguments checked there)."""
+    dev = k_cache.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return kv_evict(k_cache, v_cache, scores, block_tables, context_lens, new_tables, keep, recent)
     B = block_tables.shape[0]
     nb, bs, Hkv, D = k_cache.shape
-    row = D * k_cache.element_size()
+    size = k_cache.element_size()
+    row = D * size
     if row % 16:
         raise ValueError(f"kv_cache_evict moves rows of multiples of 16 bytes, got head_dim {D} of {k_cache.dtype}")
-    with torch.cuda.device(k_cache.device):
-        bt, cl, nt = _rows_i32(block_tables), _i32(context_lens).contiguous(), _rows_i32(new_tables)
-        lens = torch.empty(B, dtype=torch.int32, device=k_cache.device)
-        kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=k_cache.device)
-        strides = (ctypes.c_longlong * 8)(*_cache_strides("key", k_cache, 1), *_cache_strides("value", v_cache, 1), bt.stride(0),
-                                          nt.stride(0))
-        _ck(_lib().tt_kv_evict(k_cache.data_ptr(), v_cache.data_ptr(), scores.data_ptr(), bt.data_ptr(), cl.data_ptr(), nt.data_ptr(),
-                               lens.data_ptr(), kept.data_ptr(), strides, B, Hkv, bs, bt.shape[1], nt.shape[1], nb, row, keep, recent,
-                               _stream()), "tt_kv_evict")
+    bt, cl, nt = _rows_i32(block_tables), _i32(context_lens).contiguous(), _rows_i32(new_tables)
+    lens = torch.empty(B, dtype=torch.int32, device=dev)
+    kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
+    strides = (ctypes.c_longlong * 8)(*_cache_strides("key", k_cache, size, 1), *_cache_strides("value", v_cache, size, 1),
+                                      bt.stride(0), nt.stride(0))
+    _ck(_lib().tt_kv_evict(k_cache.data_ptr(), v_cache.data_ptr(), scores.data_ptr(), bt.data_ptr(), cl.data_ptr(), nt.data_ptr(),
+                           lens.data_ptr(), kept.data_ptr(), strides, B, Hkv, bs, bt.shape[1], nt.shape[1], nb, row, keep, recent,
+                           _stream_of(dev)), "tt_kv_evict")
     return lens, kept
+
+
+_LOGIT_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 
 
 def adjust_logits(logits: Tensor, tokens, lens, prompt_lens, rep, pres, freq, bias_ids, bias_values, allowed, out) -> Tensor:
     """``serving.process_logits`` on the kernels of csrc/logits.cu (arguments checked there)."""
+    dev = logits.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return adjust_logits(logits, tokens, lens, prompt_lens, rep, pres, freq, bias_ids, bias_values, allowed, out)
     B, V = logits.shape
-    with torch.cuda.device(logits.device):
-        if logits.stride(1) != 1:
-            logits = logits.contiguous()
-        if out is None:
-            out = torch.empty((B, V), dtype=logits.dtype, device=logits.device)
-        if tokens is not None and tokens.stride(-1) != 1 and tokens.shape[1] > 1:
-            tokens = tokens.contiguous()
-        # the converted forms are bound to names: they must outlive the launch
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    if out is None:
+        out = logits.new_empty((B, V))
+    # what is converted is bound to a name: it must outlive the launch
+    tok = cl = cp = ids = vals = mask = None
+    length = entries = wide = tok_row = ids_row = vals_row = mask_row = 0
+    if tokens is not None:
+        length, wide = tokens.shape[1], int(tokens.dtype == torch.int64)
+        tok = tokens if length <= 1 or tokens.stride(1) == 1 else tokens.contiguous()
+        tok_row = tok.stride(0)
         cl = None if lens is None else _i32(lens).contiguous()
         cp = None if prompt_lens is None else _i32(prompt_lens).contiguous()
-        ids = None if bias_ids is None else _rows_i32(bias_ids)
-        vals = bias_values if bias_values is None or bias_values.stride(-1) == 1 else bias_values.contiguous()
-        mask = allowed if allowed is None or allowed.stride(-1) == 1 else allowed.contiguous()
-        per_row = [p.contiguous() if torch.is_tensor(p) else None for p in (rep, pres, freq)]
-        value = [0.0 if torch.is_tensor(p) else float(p) for p in (rep, pres, freq)]
-        row = lambda t: 0 if t is None else t.stride(0)  # noqa: E731
-        strides = (ctypes.c_longlong * 6)(logits.stride(0), out.stride(0), row(tokens), row(ids), row(vals), row(mask))
-        _ck(_lib().tt_process_logits(logits.data_ptr(), out.data_ptr(), _p(tokens), int(tokens is not None and tokens.dtype == torch.int64),
-                                     _p(cl), _p(cp), *(_p(p) for p in per_row), *value, _p(ids), _p(vals),
-                                     0 if ids is None else ids.shape[1], _p(mask), strides, B, V,
-                                     0 if tokens is None else tokens.shape[1],
-                                     {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}[logits.dtype], _stream()), "tt_process_logits")
+    if bias_ids is not None:
+        entries = bias_ids.shape[1]
+        ids, vals = _rows_i32(bias_ids), bias_values if bias_values.stride(1) == 1 else bias_values.contiguous()
+        ids_row, vals_row = ids.stride(0), vals.stride(0)
+    if allowed is not None:
+        mask = allowed if allowed.stride(1) == 1 else allowed.contiguous()
+        mask_row = mask.stride(0)
+    rep_t, rep = (rep.contiguous(), 0.0) if torch.is_tensor(rep) else (None, rep)
+    pres_t, pres = (pres.contiguous(), 0.0) if torch.is_tensor(pres) else (None, pres)
+    freq_t, freq = (freq.contiguous(), 0.0) if torch.is_tensor(freq) else (None, freq)
+    strides = (ctypes.c_longlong * 6)(logits.stride(0), out.stride(0), tok_row, ids_row, vals_row, mask_row)
+    _ck(_lib().tt_process_logits(logits.data_ptr(), out.data_ptr(), _p(tok), wide, _p(cl), _p(cp), _p(rep_t), _p(pres_t), _p(freq_t),
+                                 rep, pres, freq, _p(ids), _p(vals), entries, _p(mask), strides, B, V, length,
+                                 _LOGIT_TYPES[logits.dtype], _stream_of(dev)), "tt_process_logits")
     return out
 
 

@@ -57,11 +57,15 @@ def paged_attention_decode(q, k_cache, v_cache, block_tables, context_lens, scal
     return torch.einsum("bhc,bchd->bhd", p, v).to(q.dtype)
 
 
-def _whole_numbers(t, name: str, shape: tuple, device) -> None:
-    if not torch.is_tensor(t) or t.dtype not in (torch.int32, torch.int64):
+_WHOLE = (torch.int32, torch.int64)
+
+
+def _whole_numbers(t, name: str, rows: int, dims: int, device) -> None:
+    """``t`` must hold whole numbers on ``device``, ``[rows]`` or ``[rows, any]``."""
+    if not torch.is_tensor(t) or t.dtype not in _WHOLE:
         raise TypeError(f"{name} must be an int32 or int64 tensor")
-    if t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
-        raise ValueError(f"{name} must have shape {['*' if w is None else w for w in shape]}, got {list(t.shape)}")
+    if t.dim() != dims or t.shape[0] != rows:
+        raise ValueError(f"{name} must have shape {[rows, '*'][:dims]}, got {list(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the other tensors are on {device}")
 
@@ -73,18 +77,18 @@ def _no_gradient(what: str, *tensors) -> None:
 
 def _check_cache(k_cache, v_cache, scores, block_tables, context_lens, batch: int) -> None:
     """What the ops over a paged cache have in common."""
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+    shape, dev = k_cache.shape, k_cache.device
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError(f"caches must be [num_blocks, block_size, n_kv_heads, head_dim] and alike, got {list(k_cache.shape)} and {list(v_cache.shape)}")
     if v_cache.dtype != k_cache.dtype:
         raise TypeError(f"key and value cache differ in type: {k_cache.dtype}, {v_cache.dtype}")
-    dev = k_cache.device
     if v_cache.device != dev:
         raise ValueError(f"key cache on {dev}, value cache on {v_cache.device}")
-    nb, bs, hkv, _ = k_cache.shape
-    if 0 in k_cache.shape:
-        raise ValueError(f"empty cache {list(k_cache.shape)}")
-    _whole_numbers(block_tables, "block_tables", (batch, None), dev)
-    _whole_numbers(context_lens, "context_lens", (batch,), dev)
+    nb, bs, hkv, _ = shape
+    if 0 in shape:
+        raise ValueError(f"empty cache {list(shape)}")
+    _whole_numbers(block_tables, "block_tables", batch, 2, dev)
+    _whole_numbers(context_lens, "context_lens", batch, 1, dev)
     if block_tables.shape[1] * bs >= 1 << 31:
         raise ValueError("block_tables hold 2^31 tokens or more")
     if scores is not None:
@@ -196,7 +200,7 @@ def kv_cache_evict(k_cache, v_cache, scores, block_tables, context_lens, new_tab
     nb, bs, hkv, D = k_cache.shape
     if keep < 1 or not 0 <= recent <= keep:
         raise ValueError(f"keep must be at least 1 and recent in [0, keep], got {keep} and {recent}")
-    _whole_numbers(new_tables, "new_tables", (B, None), k_cache.device)
+    _whole_numbers(new_tables, "new_tables", B, 2, k_cache.device)
     room = block_tables.shape[1] * bs
     most = min(keep, room)
     if new_tables.shape[1] * bs < most:
@@ -277,18 +281,18 @@ def process_logits(logits, tokens=None, lens=None, prompt_lens=None, *, repetiti
     pres = _setting(presence_penalty, "presence_penalty", B, dev)
     freq = _setting(frequency_penalty, "frequency_penalty", B, dev)
     if tokens is not None:
-        _whole_numbers(tokens, "tokens", (B, None), dev)
+        _whole_numbers(tokens, "tokens", B, 2, dev)
         if tokens.shape[1] > HISTORY_MAX:
             raise ValueError(f"tokens are longer than {HISTORY_MAX}")
         for t, name in ((lens, "lens"), (prompt_lens, "prompt_lens")):
             if t is not None:
-                _whole_numbers(t, name, (B,), dev)
+                _whole_numbers(t, name, B, 1, dev)
     elif lens is not None or prompt_lens is not None or any(torch.is_tensor(p) or p != d for p, d in ((rep, 1.0), (pres, 0.0), (freq, 0.0))):
         raise ValueError("penalties and lengths need tokens")
     if (bias_ids is None) != (bias_values is None):
         raise ValueError("bias_ids and bias_values go together")
     if bias_ids is not None:
-        _whole_numbers(bias_ids, "bias_ids", (B, None), dev)
+        _whole_numbers(bias_ids, "bias_ids", B, 2, dev)
         if bias_values.dtype != torch.float32 or bias_values.shape != bias_ids.shape or bias_values.device != dev:
             raise ValueError(f"bias_values must be fp32 {list(bias_ids.shape)} on {dev}")
         if bias_ids.shape[1] > LOGIT_BIASES_MAX:
