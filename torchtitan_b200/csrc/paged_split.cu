@@ -24,7 +24,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMinChunk = 512;    // tokens
-constexpr int kMaxChunks = 128;   // per sequence: bounds the workspace and the join's work
+constexpr int kMaxChunks = 256;   // per sequence: bounds the workspace and the join's work
 constexpr int kTile = 8;          // query heads of one kv head in a tile of columns
 constexpr int kMaxBatch = 2048;   // sequences of one launch (their chunk counts are kept in shared memory)
 
@@ -137,9 +137,6 @@ __device__ __forceinline__ void finish(const Args& a, int b, int h, int d, float
 constexpr int kWarps = 4;
 constexpr int kRows = 16;        // tokens of one step of a warp
 
-constexpr int kMerge = 32;        // dims of the warps' results that are merged at a time
-constexpr int kPitch = kMerge + 4;
-
 // A stage: kRows rows of K, then of V. Rows lie 16 bytes more than their length apart, so that the eight rows of a matrix
 // load touch different banks.
 template <int D> struct Ring {
@@ -148,7 +145,7 @@ template <int D> struct Ring {
   static constexpr int kBytes = kWarps * kStages * kStageBytes;
 };
 template <int D, int NT> constexpr int smem_bytes() {
-  return Ring<D>::kBytes + kWarps * kTile * kPitch * 4 + kWarps * kTile * NT * 8 + (D == 256 ? NT * (D / 16) * 32 * 8 : 0);
+  return Ring<D>::kBytes + kWarps * kTile * NT * 8 + (D == 256 ? NT * (D / 16) * 32 * 8 : 0);
 }
 
 // One piece of work: chunk c of sequence b for a tile of NT * 8 query heads of kv head hk.
@@ -159,7 +156,7 @@ struct Item {
 
 // items are numbered ((sequence, chunk), kv head, tile), the last fastest: neighbours read the same tokens' heads, which lie
 // next to each other in the cache.
-__device__ __forceinline__ void item_at(Item& it, const Args& a, const int* before, const uint8_t* counts, int hkts, int tiles, int i) {
+__device__ __forceinline__ void item_at(Item& it, const Args& a, const int* before, const uint16_t* counts, int hkts, int tiles, int i) {
   const int bc = i / hkts, hkt = i - bc * hkts;
   it.hk = hkt / tiles;
   it.tile = hkt - it.hk * tiles;
@@ -188,12 +185,11 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
   using R = Ring<D>;
   constexpr bool QS = D == 256;                   // q's fragments in shared memory: they do not fit the registers
   extern __shared__ __align__(128) unsigned char smem[];
-  float* s_o = reinterpret_cast<float*>(smem + R::kBytes);                                   // [warp][8][kPitch]
-  float2* s_ml = reinterpret_cast<float2*>(s_o + kWarps * kTile * kPitch);                  // [warp][NT * 8]
+  float2* s_ml = reinterpret_cast<float2*>(smem + R::kBytes);                                // [warp][NT * 8]
   uint2* s_q = reinterpret_cast<uint2*>(s_ml + kWarps * kTile * NT);                         // [NT][D / 16][32]
   int* before = reinterpret_cast<int*>(s_q + (QS ? NT * (D / 16) * 32 : 0));                 // [groups of 16 sequences + 1]
-  uint8_t* counts = reinterpret_cast<uint8_t*>(before + (a.B + 15) / 16 + 1);                // [B]
-  __shared__ int s_sum[kWarps];
+  uint16_t* counts = reinterpret_cast<uint16_t*>(before + (a.B + 15) / 16 + 1);                // [B]
+  __shared__ int s_sum[kWarps], s_free[kWarps];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int G = a.H / a.Hkv, tiles = (G + kTile * NT - 1) / (kTile * NT), hkts = a.Hkv * tiles;
   asm volatile("griddepcontrol.launch_dependents;");       // the join's CTAs may come up, and wait for this grid's end
@@ -206,7 +202,7 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
     for (int b = tid; b < a.B; b += 32 * kWarps) {
       const Range r = range_of(a, b);
       const int n = r.n - r.lo;
-      counts[b] = static_cast<uint8_t>(n > 0 ? (n + chunk_len(n) - 1) / chunk_len(n) : 0);
+      counts[b] = static_cast<uint16_t>(n > 0 ? (n + chunk_len(n) - 1) / chunk_len(n) : 0);
     }
     __syncthreads();
     int sum = 0;
@@ -313,37 +309,48 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
 
   const float c2 = a.scale * kLog2e;
   const int cx = 2 * (lane & 3);                  // this thread's columns (heads): cx, cx + 1 of each tile
-  Item it;
-  for (int i = blockIdx.x; i < items; i += gridDim.x) {
-    item_at(it, a, before, counts, hkts, tiles, i);
-    const int hk = it.hk, g0 = it.tile * kTile * NT, ng = min(kTile * NT, G - g0);
-    // q as the right operand: column = head, consecutive k in a register
-    uint2 qf[QS ? 1 : NT][QS ? 1 : D / 16];
-    auto q_frag = [&](int nt, int kk) {
-      const int g = nt * kTile + lane / 4;
-      uint2 v = make_uint2(0, 0);
+  // q as the right operand: column = head, consecutive k in a register. The next item and its q are fetched while the current
+  // one waits for its first tokens.
+  constexpr int QN = QS ? NT * (D / 16) / kWarps : NT * (D / 16);      // with q in shared memory each warp fetches its share
+  Item it = {}, next = {};
+  uint2 qn[QN];
+  auto fetch = [&](int i) {
+    if (i >= items) return;
+    item_at(next, a, before, counts, hkts, tiles, i);
+    const int g0 = next.tile * kTile * NT, ng = min(kTile * NT, G - g0);
+    const T* q = static_cast<const T*>(a.q) + next.b * a.q_b + (next.hk * G + g0) * a.q_h;
+#pragma unroll
+    for (int f = 0; f < QN; ++f) {
+      const int at = QS ? f * kWarps + warp : f, g = at / (D / 16) * kTile + lane / 4;
+      qn[f] = make_uint2(0, 0);
       if (g < ng) {
-        const T* qp = static_cast<const T*>(a.q) + it.b * a.q_b + (hk * G + g0 + g) * a.q_h + kk * 16 + cx;
-        v.x = *reinterpret_cast<const uint32_t*>(qp);
-        v.y = *reinterpret_cast<const uint32_t*>(qp + 8);
+        const T* qp = q + g * a.q_h + at % (D / 16) * 16 + cx;
+        qn[f].x = *reinterpret_cast<const uint32_t*>(qp);
+        qn[f].y = *reinterpret_cast<const uint32_t*>(qp + 8);
       }
-      return v;
-    };
+    }
+  };
+  fetch(blockIdx.x);
+  for (int i = blockIdx.x; i < items; i += gridDim.x) {
+    it = next;
+    const int hk = it.hk, g0 = it.tile * kTile * NT, ng = min(kTile * NT, G - g0);
+    uint2 qf[QS ? 1 : NT][QS ? 1 : D / 16];
     if constexpr (QS) {
-      __syncthreads();
-      for (int f = warp; f < NT * (D / 16); f += kWarps) s_q[f * 32 + lane] = q_frag(f / (D / 16), f % (D / 16));
-      __syncthreads();
+#pragma unroll
+      for (int f = 0; f < QN; ++f) s_q[(f * kWarps + warp) * 32 + lane] = qn[f];
+      __syncthreads();                            // the merge's barriers lie between this and the last use of the old q
     } else {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) qf[nt][kk] = q_frag(nt, kk);
+        for (int kk = 0; kk < D / 16; ++kk) qf[nt][kk] = qn[nt * (D / 16) + kk];
     }
-    float o[NT][D / 16][4], m[NT][2], l[NT][2];
+    bool fetched = false;
+    float o[NT][D / 16][4], m[NT][2], base[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
+      base[nt][0] = base[nt][1] = l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
       for (int dd = 0; dd < D / 16; ++dd)
 #pragma unroll
@@ -351,6 +358,10 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
     }
     for (int t = it.t0 + warp * kRows; t < it.t1; t += kWarps * kRows) {
       load(stage == 0 ? R::kStages - 1 : stage - 1);
+      if (!fetched) {
+        fetch(i + gridDim.x);
+        fetched = true;
+      }
       wait_group<R::kStages - 1>();
       __syncwarp();
       const uint32_t ks = ring + stage * R::kStageBytes, vs = ks + kRows * R::kRowPitch;
@@ -373,41 +384,52 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
           }
         }
       }
-      const int ta = t + lane / 4, tb = ta + 8;
-      const bool la = ta >= it.r.first && ta < it.t1, lb = tb >= it.r.first && tb < it.t1;
       uint32_t hi_p[NT][2], lo_p[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = (e < 2 ? la : lb) ? (s[nt][e] + s2[nt][e]) * c2 : -INFINITY;
-        if (a.ws_x) {
+        for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * c2;
+        if (t < it.r.first || t + kRows > it.t1) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int g = nt * kTile + cx + (e & 1), tt = e < 2 ? ta : tb;
-            if (g < ng && (e < 2 ? la : lb)) a.ws_x[((static_cast<long long>(it.b) * a.Hkv + hk) * a.span + (tt - it.r.lo)) * G + g0 + g] = s[nt][e];
+            const int tt = t + lane / 4 + (e >> 1) * 8;
+            if (tt < it.r.first || tt >= it.t1) s[nt][e] = -INFINITY;
           }
         }
-        float f[2];
+        if (a.ws_x) {
+          float* xt = a.ws_x + ((static_cast<long long>(it.b) * a.Hkv + hk) * a.span + (t - it.r.lo)) * G + g0;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float top = fmaxf(s[nt][e], s[nt][e + 2]);
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          top = fmaxf(top, m[nt][e]);
-          const float base = top == -INFINITY ? 0.f : top;
-          f[e] = ex2(m[nt][e] - base);
-          m[nt][e] = top;
-          s[nt][e] = ex2(s[nt][e] - base);
-          s[nt][e + 2] = ex2(s[nt][e + 2] - base);
-          l[nt][e] = l[nt][e] * f[e] + s[nt][e] + s[nt][e + 2];
+          for (int e = 0; e < 4; ++e) {
+            const int g = nt * kTile + cx + (e & 1), r = lane / 4 + (e >> 1) * 8;
+            if (g < ng && t + r >= it.r.first && t + r < it.t1) xt[r * G + g] = s[nt][e];
+          }
         }
-        if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+        // The exponents' base is the largest logit so far, or one at most 8 below it: it is raised (and what was summed is
+        // scaled) only when a logit is over 2^8 above it, which after the first step is rare. Weights up to 2^8 lose nothing.
+        const float big0 = fmaxf(s[nt][0], s[nt][2]), big1 = fmaxf(s[nt][1], s[nt][3]);
+        if (__any_sync(0xffffffffu, big0 > m[nt][0] + 8.f || big1 > m[nt][1] + 8.f)) {
+          float f[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = e ? big1 : big0;
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            top = fmaxf(top, m[nt][e]);
+            base[nt][e] = top == -INFINITY ? 0.f : top;
+            f[e] = ex2(m[nt][e] - base[nt][e]);
+            m[nt][e] = top;
+            l[nt][e] *= f[e];
+          }
 #pragma unroll
           for (int dd = 0; dd < D / 16; ++dd)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[nt][dd][e] *= f[e & 1];
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] = ex2(s[nt][e] - base[nt][e & 1]);
+        l[nt][0] += s[nt][0] + s[nt][2];
+        l[nt][1] += s[nt][1] + s[nt][3];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t top = pack2<T>(s[nt][2 * h], s[nt][2 * h + 1]);
@@ -433,6 +455,8 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
       stage = stage + 1 == R::kStages ? 0 : stage + 1;
     }
 
+    if (!fetched) fetch(i + gridDim.x);           // a warp without a step in this item
+
     // ---- the four warps' parts, in their order
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -445,11 +469,29 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
         if (lane < 4) s_ml[warp * kTile * NT + nt * kTile + cx + e] = make_float2(m[nt][e], x);
       }
     const long long row = static_cast<long long>(it.b) * a.chunks * a.H + static_cast<long long>(it.c) * a.H + hk * G + g0;
-    const int g = tid / 16, d = tid % 16 * 2;     // this thread's head of a tile, and its two dims of kMerge
+    // a warp's results go through the stage of its ring that waits to be filled
+    constexpr int kPitch = D + 4;                 // the rows of the four columns that a store writes lie in different banks
+    static_assert(kTile * NT * kPitch * 4 <= R::kStageBytes, "results fit a stage");
+    {
+      const int idle = stage == 0 ? R::kStages - 1 : stage - 1;
+      if (lane == 0) s_free[warp] = idle;
+      float* mine = reinterpret_cast<float*>(smem + (warp * R::kStages + idle) * R::kStageBytes);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int dd = 0; dd < D / 16; ++dd)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mine[(nt * kTile + cx + (e & 1)) * kPitch + dd * 16 + lane / 4 + (e >> 1) * 8] = o[nt][dd][e];
+    }
     __syncthreads();
+    const int d = tid % 16 * 2;                   // sixteen threads to a head, two dims of every 32 to a thread
+    const float* from[kWarps];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) from[w] = reinterpret_cast<const float*>(smem + (w * R::kStages + s_free[w]) * R::kStageBytes);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int gg = nt * kTile + g;
+      const int gg = nt * kTile + tid / 16;
+      if (gg >= ng) break;
       float top = -INFINITY, sum = 0.f, f[kWarps];
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w * kTile * NT + gg].x);
@@ -461,32 +503,24 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
         sum += y.y * f[w];            // NaN tokens leave m alone: 0 * NaN carries a sum of NaN on
       }
 #pragma unroll
-      for (int part = 0; part < D / kMerge; ++part) {
-        float* mine = s_o + warp * kTile * kPitch;
+      for (int part = 0; part < D / 32; ++part) {
+        const int at = part * 32 + d;
+        float2 x = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int dd = 0; dd < kMerge / 16; ++dd)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mine[(cx + (e & 1)) * kPitch + dd * 16 + lane / 4 + (e >> 1) * 8] = o[nt][part * (kMerge / 16) + dd][e];
-        __syncthreads();
-        if (gg < ng) {
-          float2 x = make_float2(0.f, 0.f);
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            const float2 y = *reinterpret_cast<const float2*>(s_o + (w * kTile + g) * kPitch + d);
-            x.x += y.x * f[w];
-            x.y += y.y * f[w];
-          }
-          const int at = part * kMerge + d;
-          if (it.chunks > 1) {
-            *reinterpret_cast<float2*>(a.ws_o + (row + gg) * D + at) = x;
-            if (at == 0) a.ws_ml[row + gg] = make_float2(top, sum);
-          } else {
-            finish<T, D>(a, it.b, hk * G + g0 + gg, at, top, sum, x);
-          }
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 y = *reinterpret_cast<const float2*>(from[w] + gg * kPitch + at);
+          x.x += y.x * f[w];
+          x.y += y.y * f[w];
         }
-        __syncthreads();
+        if (it.chunks > 1) {
+          *reinterpret_cast<float2*>(a.ws_o + (row + gg) * D + at) = x;
+          if (at == 0) a.ws_ml[row + gg] = make_float2(top, sum);
+        } else {
+          finish<T, D>(a, it.b, hk * G + g0 + gg, at, top, sum, x);
+        }
       }
     }
+    __syncthreads();
   }
   if (a.chunks <= 1) {                            // no join follows: sequences without tokens are answered here
     for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
@@ -497,55 +531,64 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
   }
 }
 
-// CTA = (query head, sequence): the chunks, D / 2 threads to a chunk, 512 / D of them side by side; the partial sums of the
-// rows of threads are added in their order.
+// CTA = (query head, sequence): D / 4 threads to a chunk, 1024 / D chunks side by side; the partial sums of the rows of threads
+// are added in their order.
+constexpr int kJoin = 256;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) join_kernel(const Args a) {
-  constexpr int W = D / 2, S = 256 / W;
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, d = tid % W * 2, s = tid / W;
+__global__ void __launch_bounds__(kJoin) join_kernel(const Args a) {
+  constexpr int W = D / 4, S = kJoin / W;
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid % 32, warp = tid / 32, d = tid % W * 4, s = tid / W;
   const Range r = range_of(a, b);
   const int span = r.n - r.lo, nc = span > 0 ? (span + chunk_len(span) - 1) / chunk_len(span) : 0;
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (nc == 1) return;                             // written by the split kernel
-  __shared__ float s_f[kMaxChunks], s_top[8], s_sum[8];
-  __shared__ float2 s_x[S][W];
+  __shared__ float s_f[kMaxChunks], s_top[kJoin / 32], s_sum[kJoin / 32];
+  __shared__ __align__(16) float4 s_x[S][W];
   const float2* ml = a.ws_ml + static_cast<long long>(b) * a.chunks * a.H + h;
-  const float* po = a.ws_o + (static_cast<long long>(b) * a.chunks * a.H + h) * D;
+  const float* po = a.ws_o + (static_cast<long long>(b) * a.chunks * a.H + h) * D + d;
   const float2 mine = tid < nc ? ml[static_cast<long long>(tid) * a.H] : make_float2(-INFINITY, 0.f);
   float top = mine.x;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (tid % 32 == 0) s_top[tid / 32] = top;
+  if (lane == 0) s_top[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, s_top[w]);
+  for (int w = 0; w < kMaxChunks / 32; ++w) top = fmaxf(top, s_top[w]);
   const float f = ex2(mine.x - (top == -INFINITY ? 0.f : top));
   if (tid < nc) s_f[tid] = f;
   float sum = tid < nc ? mine.y * f : 0.f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (tid % 32 == 0) s_sum[tid / 32] = sum;
+  if (lane == 0) s_sum[warp] = sum;
   __syncthreads();
-  float2 x = make_float2(0.f, 0.f);
-#pragma unroll 4
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
   for (int c = s; c < nc; c += S) {
-    const float2 y = *reinterpret_cast<const float2*>(po + static_cast<long long>(c) * a.H * D + d);
-    x.x += y.x * s_f[c];
-    x.y += y.y * s_f[c];
+    const float4 y = *reinterpret_cast<const float4*>(po + static_cast<long long>(c) * a.H * D);
+    const float g = s_f[c];
+    x.x += y.x * g;
+    x.y += y.y * g;
+    x.z += y.z * g;
+    x.w += y.w * g;
   }
   s_x[s][tid % W] = x;
   __syncthreads();
   if (s == 0) {
     sum = r.bad ? NAN : 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) sum += s_sum[w];
+    for (int w = 0; w < kMaxChunks / 32; ++w) sum += s_sum[w];
 #pragma unroll
     for (int i = 1; i < S; ++i) {
-      x.x += s_x[i][tid].x;
-      x.y += s_x[i][tid].y;
+      const float4 y = s_x[i][tid];
+      x.x += y.x;
+      x.y += y.y;
+      x.z += y.z;
+      x.w += y.w;
     }
-    finish<T, D>(a, b, h, d, top, sum, x);
+    finish<T, D>(a, b, h, d, top, sum, make_float2(x.x, x.y));
+    finish<T, D>(a, b, h, d + 2, top, sum, make_float2(x.z, x.w));
   }
 }
 
@@ -603,7 +646,7 @@ int sm_count(int dev) {
 template <typename T, int D, int NT>
 int launch(const Args& a, int dev, cudaStream_t st) {
   const int G = a.H / a.Hkv, tiles = (G + kTile * NT - 1) / (kTile * NT);
-  const int bytes = smem_bytes<D, NT>() + ((a.B + 15) / 16 + 1) * 4 + a.B;
+  const int bytes = smem_bytes<D, NT>() + ((a.B + 15) / 16 + 1) * 4 + 2 * a.B;
   if (bytes > kMostSmem) return -2;
   static std::atomic<uint64_t> ready{0};        // devices on which the kernel may take its shared memory
   if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
@@ -621,7 +664,7 @@ int launch(const Args& a, int dev, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.H, a.B);
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(kJoin);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
