@@ -134,19 +134,26 @@ __device__ __forceinline__ void finish(const Args& a, int b, int h, int d, float
   }
 }
 
-constexpr int kWarps = 4;
+constexpr int kGroups = 4;       // of warps: each takes every fourth step of a chunk
 constexpr int kRows = 16;        // tokens of one step of a warp
 
-// A stage: kRows rows of K, then of V. Rows lie 16 bytes more than their length apart, so that the eight rows of a matrix
-// load touch different banks.
-template <int D> struct Ring {
-  static constexpr int kRowBytes = 2 * D, kRowPitch = kRowBytes + 16, kStageBytes = 2 * kRows * kRowPitch;
-  static constexpr int kStages = 3;
-  static constexpr int kBytes = kWarps * kStages * kStageBytes;
+// How D dims are shared: a warp takes at most 128 of them, so that its results stay in registers; with 256, two warps of a
+// group take the same tokens, add up their halves of the logits through shared memory, and go on with half the dims each.
+template <int D> struct Shape {
+  static constexpr int kDims = D < 128 ? D : 128, kParts = D / kDims, kWarps = kGroups * kParts;
 };
-template <int D, int NT> constexpr int smem_bytes() {
-  return Ring<D>::kBytes + kWarps * kTile * NT * 8 + (D == 256 ? NT * (D / 16) * 32 * 8 : 0);
-}
+
+// A warp's stage: kRows rows of K, then of V. Rows lie 16 bytes more than their length apart, so that the eight rows of a
+// matrix load touch different banks.
+template <int D> struct Ring {
+  static constexpr int kRowBytes = 2 * Shape<D>::kDims, kRowPitch = kRowBytes + 16, kStageBytes = 2 * kRows * kRowPitch;
+  static constexpr int kStages = 3;
+  static constexpr int kBytes = Shape<D>::kWarps * kStages * kStageBytes;
+};
+template <int D, int NT> struct Exchange {     // [group][2 turns][part][NT * 4 logits][lane]
+  static constexpr int kBytes = Shape<D>::kParts > 1 ? kGroups * 2 * 2 * NT * 4 * 32 * 4 : 0;
+};
+template <int D, int NT> constexpr int smem_bytes() { return Ring<D>::kBytes + kGroups * kTile * NT * 8 + Exchange<D, NT>::kBytes; }
 
 // One piece of work: chunk c of sequence b for a tile of NT * 8 query heads of kv head hk.
 struct Item {
@@ -179,18 +186,20 @@ __device__ __forceinline__ void item_at(Item& it, const Args& a, const int* befo
 // Tokens as rows of the products' left operand, query heads as columns: S^T = K q^T and O^T += V^T P^T, eight query heads
 // being one tile of columns, so that groups of up to 8 heads waste nothing. P is passed as its rounding to T plus the
 // rounding of the remainder, which keeps 16 bits of it (P in T alone would add an error as large as the output's own
-// rounding). A warp owns every fourth 16 tokens of a chunk and a ring of stages; its loads run ahead across chunks.
+// rounding). A group of warps (one, or two with 256 dims)
+// owns every fourth 16 tokens of a chunk; every warp has a ring of stages, and its loads run ahead across chunks.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args a) {
   using R = Ring<D>;
-  constexpr bool QS = D == 256;                   // q's fragments in shared memory: they do not fit the registers
+  constexpr int kExchange = Exchange<D, NT>::kBytes;
+  constexpr int DW = Shape<D>::kDims, DP = Shape<D>::kParts, kWarps = Shape<D>::kWarps;
   extern __shared__ __align__(128) unsigned char smem[];
-  float2* s_ml = reinterpret_cast<float2*>(smem + R::kBytes);                                // [warp][NT * 8]
-  uint2* s_q = reinterpret_cast<uint2*>(s_ml + kWarps * kTile * NT);                         // [NT][D / 16][32]
-  int* before = reinterpret_cast<int*>(s_q + (QS ? NT * (D / 16) * 32 : 0));                 // [groups of 16 sequences + 1]
-  uint16_t* counts = reinterpret_cast<uint16_t*>(before + (a.B + 15) / 16 + 1);                // [B]
+  float2* s_ml = reinterpret_cast<float2*>(smem + R::kBytes);                                // [group][NT * 8]
+  float* s_x = reinterpret_cast<float*>(s_ml + kGroups * kTile * NT);                        // [group][2][part][NT * 4][lane]
+  int* before = reinterpret_cast<int*>(reinterpret_cast<char*>(s_x) + kExchange);   // [groups of 16 sequences + 1]
+  uint16_t* counts = reinterpret_cast<uint16_t*>(before + (a.B + 15) / 16 + 1);           // [B]
   __shared__ int s_sum[kWarps], s_free[kWarps];
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, group = warp / DP, part = warp % DP;
   const int G = a.H / a.Hkv, tiles = (G + kTile * NT - 1) / (kTile * NT), hkts = a.Hkv * tiles;
   asm volatile("griddepcontrol.launch_dependents;");       // the join's CTAs may come up, and wait for this grid's end
 
@@ -226,8 +235,8 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
   }
   const int items = before[(a.B + 15) / 16] * hkts;
   const uint32_t ring = smem_u32(smem) + warp * R::kStages * R::kStageBytes;
-  const T* kc = static_cast<const T*>(a.k);
-  const T* vc = static_cast<const T*>(a.v);
+  const T* kc = static_cast<const T*>(a.k) + part * DW;
+  const T* vc = static_cast<const T*>(a.v) + part * DW;
 
   // ---- the loads: `head` is the item being loaded, ht its next token, page its table entry for row lane % 16
   Item head = {};
@@ -243,7 +252,7 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
   };
   auto enter = [&]() {
     item_at(head, a, before, counts, hkts, tiles, hi);
-    ht = head.t0 + warp * kRows;
+    ht = head.t0 + group * kRows;
     k_head = kc + head.hk * a.k_head;
     v_head = vc + head.hk * a.v_head;
   };
@@ -258,8 +267,8 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
     enter();
     settle();
   }
-  // A lane copies 16 bytes of every (256 / D)-th row, of keys and of values; one commit group, empty when nothing is left.
-  constexpr int CH = D / 8, RPI = 32 / CH;        // 16-byte pieces of a row, rows of one copy instruction
+  // A lane copies 16 bytes of every (256 / DW)-th row, of keys and of values; one commit group, empty when nothing is left.
+  constexpr int CH = DW / 8, RPI = 32 / CH;        // 16-byte pieces of a row, rows of one copy instruction
   const int ch = lane % CH, row0 = lane / CH;
   auto load = [&](int stage) {
     if (hi < items) {
@@ -298,7 +307,7 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
           dst += RPI * R::kRowPitch;
         }
       }
-      ht += kWarps * kRows;
+      ht += kGroups * kRows;
       settle();
     }
     commit();
@@ -311,52 +320,49 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
   const int cx = 2 * (lane & 3);                  // this thread's columns (heads): cx, cx + 1 of each tile
   // q as the right operand: column = head, consecutive k in a register. The next item and its q are fetched while the current
   // one waits for its first tokens.
-  constexpr int QN = QS ? NT * (D / 16) / kWarps : NT * (D / 16);      // with q in shared memory each warp fetches its share
   Item it = {}, next = {};
-  uint2 qn[QN];
+  uint2 qn[NT][DW / 16];
   auto fetch = [&](int i) {
     if (i >= items) return;
     item_at(next, a, before, counts, hkts, tiles, i);
     const int g0 = next.tile * kTile * NT, ng = min(kTile * NT, G - g0);
-    const T* q = static_cast<const T*>(a.q) + next.b * a.q_b + (next.hk * G + g0) * a.q_h;
+    const T* q = static_cast<const T*>(a.q) + next.b * a.q_b + (next.hk * G + g0) * a.q_h + part * DW + cx;
 #pragma unroll
-    for (int f = 0; f < QN; ++f) {
-      const int at = QS ? f * kWarps + warp : f, g = at / (D / 16) * kTile + lane / 4;
-      qn[f] = make_uint2(0, 0);
-      if (g < ng) {
-        const T* qp = q + g * a.q_h + at % (D / 16) * 16 + cx;
-        qn[f].x = *reinterpret_cast<const uint32_t*>(qp);
-        qn[f].y = *reinterpret_cast<const uint32_t*>(qp + 8);
+    for (int nt = 0; nt < NT; ++nt) {
+      const int g = nt * kTile + lane / 4;
+#pragma unroll
+      for (int kk = 0; kk < DW / 16; ++kk) {
+        qn[nt][kk] = make_uint2(0, 0);
+        if (g < ng) {
+          const T* qp = q + g * a.q_h + kk * 16;
+          qn[nt][kk].x = *reinterpret_cast<const uint32_t*>(qp);
+          qn[nt][kk].y = *reinterpret_cast<const uint32_t*>(qp + 8);
+        }
       }
     }
   };
+  int turn = 0;                                   // of the exchange's two buffers
   fetch(blockIdx.x);
   for (int i = blockIdx.x; i < items; i += gridDim.x) {
     it = next;
     const int hk = it.hk, g0 = it.tile * kTile * NT, ng = min(kTile * NT, G - g0);
-    uint2 qf[QS ? 1 : NT][QS ? 1 : D / 16];
-    if constexpr (QS) {
+    uint2 qf[NT][DW / 16];
 #pragma unroll
-      for (int f = 0; f < QN; ++f) s_q[(f * kWarps + warp) * 32 + lane] = qn[f];
-      __syncthreads();                            // the merge's barriers lie between this and the last use of the old q
-    } else {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) qf[nt][kk] = qn[nt * (D / 16) + kk];
-    }
+      for (int kk = 0; kk < DW / 16; ++kk) qf[nt][kk] = qn[nt][kk];
     bool fetched = false;
-    float o[NT][D / 16][4], m[NT][2], base[NT][2], l[NT][2];
+    float o[NT][DW / 16][4], m[NT][2], base[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
       base[nt][0] = base[nt][1] = l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-      for (int dd = 0; dd < D / 16; ++dd)
+      for (int dd = 0; dd < DW / 16; ++dd)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][dd][e] = 0.f;
     }
-    for (int t = it.t0 + warp * kRows; t < it.t1; t += kWarps * kRows) {
+    for (int t = it.t0 + group * kRows; t < it.t1; t += kGroups * kRows) {
       load(stage == 0 ? R::kStages - 1 : stage - 1);
       if (!fetched) {
         fetch(i + gridDim.x);
@@ -373,22 +379,34 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
       {
         const uint32_t at = ks + (lane & 15) * R::kRowPitch + (lane >> 4) * 16;
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
+        for (int kk = 0; kk < DW / 16; ++kk) {
           uint32_t kf[4];
           ldm4(kf, at + kk * 32);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            uint2 qv;
-            if constexpr (QS) qv = s_q[(nt * (D / 16) + kk) * 32 + lane]; else qv = qf[nt][kk];
-            mma<T>(kk & 1 ? s2[nt] : s[nt], kf, qv.x, qv.y);
+            mma<T>(kk & 1 ? s2[nt] : s[nt], kf, qf[nt][kk].x, qf[nt][kk].y);
           }
         }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
+      if constexpr (DP == 2) {
+        // the other half of the dims; a buffer is written again two steps later, past another meeting
+        float* buf = s_x + ((group * 2 + turn) * 2) * NT * 4 * 32 + lane;
+#pragma unroll
+        for (int j = 0; j < NT * 4; ++j) buf[(part * NT * 4 + j) * 32] = s[j / 4][j % 4];
+        asm volatile("bar.sync %0, 64;" ::"r"(1 + group) : "memory");
+#pragma unroll
+        for (int j = 0; j < NT * 4; ++j) s[j / 4][j % 4] += buf[((part ^ 1) * NT * 4 + j) * 32];
+        turn ^= 1;
       }
       uint32_t hi_p[NT][2], lo_p[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * c2;
+        for (int e = 0; e < 4; ++e) s[nt][e] *= c2;
         if (t < it.r.first || t + kRows > it.t1) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -396,7 +414,7 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
             if (tt < it.r.first || tt >= it.t1) s[nt][e] = -INFINITY;
           }
         }
-        if (a.ws_x) {
+        if (a.ws_x && part == 0) {
           float* xt = a.ws_x + ((static_cast<long long>(it.b) * a.Hkv + hk) * a.span + (t - it.r.lo)) * G + g0;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -422,7 +440,7 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
             l[nt][e] *= f[e];
           }
 #pragma unroll
-          for (int dd = 0; dd < D / 16; ++dd)
+          for (int dd = 0; dd < DW / 16; ++dd)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[nt][dd][e] *= f[e & 1];
         }
@@ -441,7 +459,7 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
       {
         const uint32_t at = vs + ((lane & 7) + ((lane >> 4) << 3)) * R::kRowPitch + ((lane >> 3) & 1) * 16;
 #pragma unroll
-        for (int dd = 0; dd < D / 16; ++dd) {
+        for (int dd = 0; dd < DW / 16; ++dd) {
           uint32_t vf[4];
           ldm4t(vf, at + dd * 32);
 #pragma unroll
@@ -457,7 +475,7 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
 
     if (!fetched) fetch(i + gridDim.x);           // a warp without a step in this item
 
-    // ---- the four warps' parts, in their order
+    // ---- the four groups' results, in their order
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -466,11 +484,11 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
         x += __shfl_xor_sync(0xffffffffu, x, 4);
         x += __shfl_xor_sync(0xffffffffu, x, 8);
         x += __shfl_xor_sync(0xffffffffu, x, 16);
-        if (lane < 4) s_ml[warp * kTile * NT + nt * kTile + cx + e] = make_float2(m[nt][e], x);
+        if (lane < 4 && part == 0) s_ml[group * kTile * NT + nt * kTile + cx + e] = make_float2(m[nt][e], x);
       }
     const long long row = static_cast<long long>(it.b) * a.chunks * a.H + static_cast<long long>(it.c) * a.H + hk * G + g0;
     // a warp's results go through the stage of its ring that waits to be filled
-    constexpr int kPitch = D + 4;                 // the rows of the four columns that a store writes lie in different banks
+    constexpr int kPitch = DW + 4;                // the rows of the four columns that a store writes lie in different banks
     static_assert(kTile * NT * kPitch * 4 <= R::kStageBytes, "results fit a stage");
     {
       const int idle = stage == 0 ? R::kStages - 1 : stage - 1;
@@ -479,44 +497,46 @@ __global__ void __launch_bounds__(32 * kWarps) split_kernel(const Args a) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int dd = 0; dd < D / 16; ++dd)
+        for (int dd = 0; dd < DW / 16; ++dd)
 #pragma unroll
           for (int e = 0; e < 4; ++e) mine[(nt * kTile + cx + (e & 1)) * kPitch + dd * 16 + lane / 4 + (e >> 1) * 8] = o[nt][dd][e];
     }
     __syncthreads();
-    const int d = tid % 16 * 2;                   // sixteen threads to a head, two dims of every 32 to a thread
-    const float* from[kWarps];
+    // 128 threads to a part: sixteen to a head, two dims of every 32 to a thread
+    const int mp = tid / 128, mh = tid % 128 / 16, d = tid % 16 * 2;
+    const float* from[kGroups];
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) from[w] = reinterpret_cast<const float*>(smem + (w * R::kStages + s_free[w]) * R::kStageBytes);
+    for (int w = 0; w < kGroups; ++w)
+      from[w] = reinterpret_cast<const float*>(smem + ((w * DP + mp) * R::kStages + s_free[w * DP + mp]) * R::kStageBytes);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int gg = nt * kTile + tid / 16;
+      const int gg = nt * kTile + mh;
       if (gg >= ng) break;
-      float top = -INFINITY, sum = 0.f, f[kWarps];
+      float top = -INFINITY, sum = 0.f, f[kGroups];
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w * kTile * NT + gg].x);
-      const float base = top == -INFINITY ? 0.f : top;
+      for (int w = 0; w < kGroups; ++w) top = fmaxf(top, s_ml[w * kTile * NT + gg].x);
+      const float from_top = top == -INFINITY ? 0.f : top;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
+      for (int w = 0; w < kGroups; ++w) {
         const float2 y = s_ml[w * kTile * NT + gg];
-        f[w] = ex2(y.x - base);
+        f[w] = ex2(y.x - from_top);
         sum += y.y * f[w];            // NaN tokens leave m alone: 0 * NaN carries a sum of NaN on
       }
 #pragma unroll
-      for (int part = 0; part < D / 32; ++part) {
-        const int at = part * 32 + d;
+      for (int j = 0; j < DW / 32; ++j) {
+        const int at = j * 32 + d, dim = mp * DW + at;
         float2 x = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < kGroups; ++w) {
           const float2 y = *reinterpret_cast<const float2*>(from[w] + gg * kPitch + at);
           x.x += y.x * f[w];
           x.y += y.y * f[w];
         }
         if (it.chunks > 1) {
-          *reinterpret_cast<float2*>(a.ws_o + (row + gg) * D + at) = x;
-          if (at == 0) a.ws_ml[row + gg] = make_float2(top, sum);
+          if (dim == 0) a.ws_ml[row + gg] = make_float2(top, sum);
+          *reinterpret_cast<float2*>(a.ws_o + (row + gg) * D + dim) = x;
         } else {
-          finish<T, D>(a, it.b, hk * G + g0 + gg, at, top, sum, x);
+          finish<T, D>(a, it.b, hk * G + g0 + gg, dim, top, sum, x);
         }
       }
     }
@@ -656,8 +676,7 @@ int launch(const Args& a, int dev, cudaStream_t st) {
   const long long most = static_cast<long long>(a.B) * a.chunks * a.Hkv * tiles;
   const int per_sm = 228 * 1024 / (bytes + 1024);
   const long long grid = static_cast<long long>(sm_count(dev)) * (per_sm > 0 ? per_sm : 1);
-  split_kernel<T, D, NT><<<static_cast<unsigned>(most < 1 ? 1 : most < grid ? most : grid), 32 * kWarps, bytes, st>>>(a);
-  if (a.chunks <= 1 && !a.scores) return cudaGetLastError() == cudaSuccess ? 0 : -4;
+  split_kernel<T, D, NT><<<static_cast<unsigned>(most < 1 ? 1 : most < grid ? most : grid), 32 * Shape<D>::kWarps, bytes, st>>>(a);
   // these come up while the kernel before them runs, and wait for its end (griddepcontrol.wait) before they touch its results
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -668,6 +687,7 @@ int launch(const Args& a, int dev, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (a.chunks <= 1 && !a.scores) return cudaGetLastError() == cudaSuccess ? 0 : -4;
   if (a.chunks > 1 && cudaLaunchKernelEx(&cfg, join_kernel<T, D>, a) != cudaSuccess) return -4;
   if (a.scores && a.chunks > 0) {
     cfg.gridDim = dim3(a.chunks, a.Hkv, a.B);

@@ -1057,19 +1057,18 @@ def paged_split(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tenso
     chunks = L.tt_paged_split_chunks(room, win)
     out = q.new_empty((B, H, D))
     lse = torch.empty((B, H), dtype=torch.float32, device=dev) if return_lse else None
-    o = x = ml = tot = None
+    o = ml = tot = x = None
     if chunks > 1 or scores is not None:
-        # one allocation: partial outputs, every logit, the partial (maximum, sum) and the joint ones
+        # one allocation: partial outputs, their (maximum, sum), and with scores the joint ones and every logit
         rows = B * H
         n_o, n_ml = (rows * chunks * D, 2 * rows * chunks) if chunks > 1 else (0, 0)
-        n_x = rows * span + rows * span % 2 if scores is not None else 0         # pairs follow: an even number
-        ws = torch.empty(n_o + n_x + n_ml + (2 * rows if n_x else 0), dtype=torch.float32, device=dev)
+        n_tot, n_x = (2 * rows + 2, rows * span) if scores is not None else (0, 0)
+        ws = torch.empty(n_o + n_ml + n_tot + n_x, dtype=torch.float32, device=dev)
         o = ws.data_ptr()
-        x = o + 4 * n_o
-        ml = x + 4 * n_x
-        tot = ml + 4 * n_ml
-        if not n_x:
-            x = tot = None
+        ml = o + 4 * n_o
+        if n_tot:
+            tot = ml + 4 * n_ml
+            x = tot + 8 * rows + (tot + 8 * rows) % 16                             # on a 16-byte boundary
     strides = (ctypes.c_longlong * 9)(q_b, q_h, *_cache_strides("key", k_cache, 2, 2), *_cache_strides("value", v_cache, 2, 2),
                                       bt.stride(0))
     _ck(L.tt_paged_split(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), bt.data_ptr(), cl.data_ptr(), out.data_ptr(),
