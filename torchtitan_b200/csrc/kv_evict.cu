@@ -267,10 +267,14 @@ __global__ void __launch_bounds__(256) move_kernel(const Args a) {
 
 extern "C" {
 
-// strides in bytes: k (page, token, head), v (page, token, head), then in elements: table row, new table row.
-int tt_kv_evict(void* k, void* v, float* scores, const int* tables, const int* lens, const int* fresh, int* new_lens, int* kept,
-                const long long* strides, int B, int Hkv, int page, int width, int fresh_width, int pages, int row_bytes, int keep,
-                int recent, cudaStream_t st) {
+// v: the arguments as 64-bit words in the order of the names below; cache strides in bytes, table strides in elements.
+int tt_kv_evict(const long long* v, cudaStream_t st) {
+  enum { K, V, SCORES, TABLES, LENS, FRESH, NEW_LENS, KEPT, K_PAGE, K_TOK, K_HEAD, V_PAGE, V_TOK, V_HEAD, TABLE_ROW, FRESH_ROW, BATCH,
+         KV_HEADS, PAGE, WIDTH, FRESH_WIDTH, PAGES, ROW_BYTES, KEEP, RECENT };
+  auto at = [&](int i) { return reinterpret_cast<void*>(v[i]); };
+  auto num = [&](int i) { return static_cast<int>(v[i]); };
+  const int B = num(BATCH), Hkv = num(KV_HEADS), page = num(PAGE), width = num(WIDTH), fresh_width = num(FRESH_WIDTH), pages = num(PAGES),
+            row_bytes = num(ROW_BYTES), keep = num(KEEP), recent = num(RECENT);
   if (B <= 0 || Hkv <= 0) return 0;
   if (B > 65535 || row_bytes % 16 || keep < 1 || recent < 0 || recent > keep) return -2;
   const long long room = static_cast<long long>(width) * page, most = room < keep ? room : keep;
@@ -280,8 +284,9 @@ int tt_kv_evict(void* k, void* v, float* scores, const int* tables, const int* l
   while (parts < kMostParts && static_cast<long long>(B) * Hkv * parts < 148 && room / (2 * parts) >= 2048) parts *= 2;
   const long long per = (room + parts - 1) / parts;
   const int held = static_cast<int>(per < kMostHeld ? per : kMostHeld);
-  Args a{static_cast<char*>(k), static_cast<char*>(v), scores, tables, lens, fresh, new_lens, kept,
-         strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7],
+  Args a{static_cast<char*>(at(K)), static_cast<char*>(at(V)), static_cast<float*>(at(SCORES)), static_cast<const int*>(at(TABLES)),
+         static_cast<const int*>(at(LENS)), static_cast<const int*>(at(FRESH)), static_cast<int*>(at(NEW_LENS)),
+         static_cast<int*>(at(KEPT)), v[K_PAGE], v[K_TOK], v[K_HEAD], v[V_PAGE], v[V_TOK], v[V_HEAD], v[TABLE_ROW], v[FRESH_ROW],
          B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held, page & (page - 1) ? -1 : __builtin_ctz(page)};
   static std::atomic<uint64_t> ready{0};          // devices on which the kernel may take its shared memory
   int dev = 0;

@@ -235,15 +235,39 @@ int launch(Args a, int B, cudaStream_t st) {
 
 extern "C" {
 
-// dtype: 0 = bf16, 1 = fp32, 2 = fp16. strides (elements): x row, y row, tokens row, bias ids row, bias values row, mask row.
-int tt_process_logits(const void* x, void* y, const void* tokens, int tok64, const int* lens, const int* prompts, const float* rep_t,
-                      const float* pres_t, const float* freq_t, float rep, float pres, float freq, const int* bias_ids,
-                      const float* bias_values, int nb, const int* allowed, const long long* strides, int B, int V, int L, int dtype,
-                      cudaStream_t st) {
-  if (B <= 0 || V <= 0) return 0;
-  if (nb > kMaxBias || L > static_cast<int>(kCount) || B > 65535 || V >= 1 << 30) return -2;
-  Args a{x, y, tokens, lens, prompts, rep_t, pres_t, freq_t, bias_ids, bias_values, allowed,
-         strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], V, L, nb, tok64, 0, rep, pres, freq};
+// v: the arguments as 64-bit words in the order of the names below; strides in elements. dtype: 0 = bf16, 1 = fp32, 2 = fp16.
+int tt_process_logits(const long long* v, float rep, float pres, float freq, cudaStream_t st) {
+  enum { X, Y, TOKENS, LENS, PROMPTS, REP, PRES, FREQ, BIAS_IDS, BIAS_VALUES, ALLOWED, X_ROW, Y_ROW, TOK_ROW, ID_ROW, VAL_ROW, MASK_ROW,
+         TOK64, ENTRIES, BATCH, VOCAB, LENGTH, DTYPE };
+  auto at = [&](int i) { return reinterpret_cast<void*>(v[i]); };
+  const int B = static_cast<int>(v[BATCH]), dtype = static_cast<int>(v[DTYPE]);
+  if (B <= 0 || v[VOCAB] <= 0) return 0;
+  if (v[ENTRIES] > kMaxBias || v[LENGTH] > static_cast<int>(kCount) || B > 65535 || v[VOCAB] >= 1 << 30) return -2;
+  Args a = {};
+  a.x = at(X);
+  a.y = at(Y);
+  a.tokens = at(TOKENS);
+  a.lens = static_cast<const int*>(at(LENS));
+  a.prompts = static_cast<const int*>(at(PROMPTS));
+  a.rep_t = static_cast<const float*>(at(REP));
+  a.pres_t = static_cast<const float*>(at(PRES));
+  a.freq_t = static_cast<const float*>(at(FREQ));
+  a.bias_ids = static_cast<const int*>(at(BIAS_IDS));
+  a.bias_values = static_cast<const float*>(at(BIAS_VALUES));
+  a.allowed = static_cast<const int*>(at(ALLOWED));
+  a.x_row = v[X_ROW];
+  a.y_row = v[Y_ROW];
+  a.tok_row = v[TOK_ROW];
+  a.id_row = v[ID_ROW];
+  a.val_row = v[VAL_ROW];
+  a.mask_row = v[MASK_ROW];
+  a.V = static_cast<int>(v[VOCAB]);
+  a.L = static_cast<int>(v[LENGTH]);
+  a.nb = static_cast<int>(v[ENTRIES]);
+  a.tok64 = static_cast<int>(v[TOK64]);
+  a.rep = rep;
+  a.pres = pres;
+  a.freq = freq;
   if (dtype == 0) return launch<__nv_bfloat16>(a, B, st);
   if (dtype == 1) return launch<float>(a, B, st);
   if (dtype == 2) return launch<__half>(a, B, st);

@@ -701,27 +701,59 @@ int launch(const Args& a, int dev, cudaStream_t st) {
 
 extern "C" {
 
-// Chunks that a sequence of at most `tokens` live tokens (its window, where there is one) can be cut into, and the tokens
-// that are read for it: the sizes of the workspaces.
-int tt_paged_split_chunks(int tokens, int window) {
-  const int span = window > 0 && window + 15 < tokens ? window + 15 : tokens;
-  const int c = (span + kMinChunk - 1) / kMinChunk;
-  return c < kMaxChunks ? c : kMaxChunks;
-}
+// The chunk rule's numbers, for the size of the workspaces: a sequence of at most n live tokens (its window + 15, where there
+// is one) is cut into at most min(most, ceil(n / least)) chunks.
+int tt_paged_split_least_chunk() { return kMinChunk; }
+int tt_paged_split_most_chunks() { return kMaxChunks; }
 
-// dtype: 0 = bf16, 2 = fp16. strides: q (sequence, head), k (page, token, head), v (page, token, head), table row.
-int tt_paged_split(const void* q, const void* k, const void* v, const int* tables, const int* lens, void* out, float* lse,
-                   const float* sinks, float* scores, float* ws_o, void* ws_ml, void* ws_tot, float* ws_x,
-                   const long long* strides, int B, int H, int Hkv, int D, int page, int width, int pages, int window, int span,
-                   int chunks, float scale, int dtype, cudaStream_t st) {
+// v: the arguments as 64-bit words -- addresses, whole numbers, strides in elements -- in the order of the names below. One
+// block instead of some thirty arguments: a call from Python spends its time on those. dtype: 0 = bf16, 2 = fp16.
+int tt_paged_split(const long long* v, float scale, cudaStream_t st) {
+  enum { Q, K, V, TABLES, LENS, OUT, LSE, SINKS, SCORES, WS_O, WS_ML, WS_TOT, WS_X, Q_B, Q_H, K_PAGE, K_TOK, K_HEAD, V_PAGE, V_TOK,
+         V_HEAD, TABLE_ROW, BATCH, HEADS, KV_HEADS, DIM, PAGE, WIDTH, PAGES, WINDOW, SPAN, CHUNKS, DTYPE };
+  auto at = [&](int i) { return reinterpret_cast<void*>(v[i]); };
+  auto num = [&](int i) { return static_cast<int>(v[i]); };
+  const int B = num(BATCH), H = num(HEADS), Hkv = num(KV_HEADS), D = num(DIM), page = num(PAGE), dtype = num(DTYPE);
   if (B <= 0 || H <= 0) return 0;
   if (Hkv <= 0 || H % Hkv) return -12;
   if (B > kMaxBatch) return -2;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -4;
-  Args a{q, k, v, tables, lens, out, lse, sinks, scores, ws_o, static_cast<float2*>(ws_ml), static_cast<float2*>(ws_tot), ws_x,
-         strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6], strides[7], strides[8],
-         B, H, Hkv, page, width, pages, window, span, chunks, page & (page - 1) ? -1 : __builtin_ctz(page), page % 8 == 0, scale};
+  Args a = {};
+  a.q = at(Q);
+  a.k = at(K);
+  a.v = at(V);
+  a.tables = static_cast<const int*>(at(TABLES));
+  a.lens = static_cast<const int*>(at(LENS));
+  a.out = at(OUT);
+  a.lse = static_cast<float*>(at(LSE));
+  a.sinks = static_cast<const float*>(at(SINKS));
+  a.scores = static_cast<float*>(at(SCORES));
+  a.ws_o = static_cast<float*>(at(WS_O));
+  a.ws_ml = static_cast<float2*>(at(WS_ML));
+  a.ws_tot = static_cast<float2*>(at(WS_TOT));
+  a.ws_x = static_cast<float*>(at(WS_X));
+  a.q_b = v[Q_B];
+  a.q_h = v[Q_H];
+  a.k_page = v[K_PAGE];
+  a.k_tok = v[K_TOK];
+  a.k_head = v[K_HEAD];
+  a.v_page = v[V_PAGE];
+  a.v_tok = v[V_TOK];
+  a.v_head = v[V_HEAD];
+  a.table_row = v[TABLE_ROW];
+  a.B = B;
+  a.H = H;
+  a.Hkv = Hkv;
+  a.page = page;
+  a.width = num(WIDTH);
+  a.pages = num(PAGES);
+  a.window = num(WINDOW);
+  a.span = num(SPAN);
+  a.chunks = num(CHUNKS);
+  a.page_shift = page & (page - 1) ? -1 : __builtin_ctz(page);
+  a.whole = page % 8 == 0;
+  a.scale = scale;
 #define PICK(T)                                   \
   switch (D) {                                    \
     case 64: return H / Hkv > kTile ? launch<T, 64, 2>(a, dev, st) : launch<T, 64, 1>(a, dev, st);     \

@@ -11,8 +11,9 @@ so once in the log.
 
 from __future__ import annotations
 
-import ctypes
+import functools
 import math
+import struct
 
 import torch
 from torch import Tensor
@@ -1018,14 +1019,25 @@ def _rows_i32(t: Tensor) -> Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _cache_strides(name: str, t: Tensor, size: int, unit: int) -> tuple:
-    """(page, token, head) strides in units of ``unit`` bytes of a cache whose heads are contiguous on 16-byte boundaries."""
-    page, tok, head, one = t.stride()
-    if 1 in t.shape:        # what is not stepped over may have any stride
-        page, tok, head = (s if n > 1 else 0 for s, n in zip((page, tok, head), t.shape))
-    if one != 1 or (t.data_ptr() | page * size | tok * size | head * size) % 16:
-        raise ValueError(f"{name} cache: heads must be contiguous and start on 16-byte boundaries (strides {t.stride()})")
-    return page * size // unit, tok * size // unit, head * size // unit
+def _cache_strides(k: Tensor, v: Tensor, size: int, unit: int) -> tuple:
+    """(page, token, head) strides of both caches in units of ``unit`` bytes; heads must be contiguous on 16-byte boundaries."""
+    ks, vs = k.stride(), v.stride()
+    if 1 in k.shape:        # what is not stepped over may have any stride
+        ks, vs = ((*(s if n > 1 else 0 for s, n in zip(x[:3], k.shape)), x[3]) for x in (ks, vs))
+    if ks[3] != 1 or vs[3] != 1 or (k.data_ptr() | v.data_ptr() | (ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) * size) % 16:
+        raise ValueError(f"caches: heads must be contiguous and start on 16-byte boundaries (strides {k.stride()}, {v.stride()})")
+    if unit == size:
+        return ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]
+    return ks[0] * size, ks[1] * size, ks[2] * size, vs[0] * size, vs[1] * size, vs[2] * size
+
+
+# the argument blocks of csrc/{paged_split,kv_evict,logits}.cu: 64-bit words
+_SPLIT_ARGS, _EVICT_ARGS, _LOGIT_ARGS = struct.Struct("33q"), struct.Struct("25q"), struct.Struct("23q")
+
+
+@functools.cache
+def _split_rule() -> tuple:
+    return _lib().tt_paged_split_least_chunk(), _lib().tt_paged_split_most_chunks()
 
 
 def paged_split(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tensor, context_lens: Tensor, scale: float, window, sinks,
@@ -1041,7 +1053,7 @@ def paged_split(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tenso
                                for t in (q, k_cache, v_cache, block_tables, context_lens)), scale, window, sinks, scores, return_lse)
                  for i in range(0, B, _PAGED_SPLIT_BATCH)]
         return tuple(torch.cat(p) for p in zip(*parts)) if return_lse else torch.cat(parts)
-    nb, bs, Hkv, _ = k_cache.shape
+    pages, page, Hkv, _ = k_cache.shape
     q_b, q_h, q_d = q.stride()
     if q_d != 1 or (q.data_ptr() | 2 * q_b | 2 * q_h) % 4:      # read two elements at a time
         q = q.clone(memory_format=torch.contiguous_format)
@@ -1049,15 +1061,15 @@ def paged_split(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tenso
     bt, cl = _rows_i32(block_tables), _i32(context_lens).contiguous()
     if sinks is not None:
         sinks = sinks.to(torch.float32).contiguous()
-    L = _lib()
     width = bt.shape[1]
-    room = width * bs
+    room = width * page
     win = 0 if window is None or window >= room else int(window)
     span = min(room, win + 15) if win else room
-    chunks = L.tt_paged_split_chunks(room, win)
+    least, most = _split_rule()
+    chunks = min(most, -(-span // least))
     out = q.new_empty((B, H, D))
     lse = torch.empty((B, H), dtype=torch.float32, device=dev) if return_lse else None
-    o = ml = tot = x = None
+    o = ml = tot = x = 0
     if chunks > 1 or scores is not None:
         # one allocation: partial outputs, their (maximum, sum), and with scores the joint ones and every logit
         rows = B * H
@@ -1069,12 +1081,12 @@ def paged_split(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tenso
         if n_tot:
             tot = ml + 4 * n_ml
             x = tot + 8 * rows + (tot + 8 * rows) % 16                             # on a 16-byte boundary
-    strides = (ctypes.c_longlong * 9)(q_b, q_h, *_cache_strides("key", k_cache, 2, 2), *_cache_strides("value", v_cache, 2, 2),
-                                      bt.stride(0))
-    _ck(L.tt_paged_split(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), bt.data_ptr(), cl.data_ptr(), out.data_ptr(),
-                         _p(lse), _p(sinks), _p(scores), o, ml, tot, x, strides,
-                         B, H, Hkv, D, bs, width, nb, win, span, chunks, scale, 0 if q.dtype == torch.bfloat16 else 2,
-                         _stream_of(dev)), "tt_paged_split")
+    args = _SPLIT_ARGS.pack(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), bt.data_ptr(), cl.data_ptr(), out.data_ptr(),
+        lse.data_ptr() if return_lse else 0, sinks.data_ptr() if sinks is not None else 0, scores.data_ptr() if scores is not None else 0,
+        o, ml, tot, x, q_b, q_h, *_cache_strides(k_cache, v_cache, 2, 2), bt.stride(0), B, H, Hkv, D, page, width, pages, win, span,
+        chunks, 0 if q.dtype == torch.bfloat16 else 2)
+    _ck(_lib().tt_paged_split(args, scale, _stream_of(dev)), "tt_paged_split")
     return (out, lse) if return_lse else out
 
 
@@ -1085,8 +1097,8 @@ def kv_evict(k_cache: Tensor, v_cache: Tensor, scores: Tensor, block_tables: Ten
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return kv_evict(k_cache, v_cache, scores, block_tables, context_lens, new_tables, keep, recent)
-    B = block_tables.shape[0]
-    nb, bs, Hkv, D = k_cache.shape
+    B, width = block_tables.shape
+    pages, page, Hkv, D = k_cache.shape
     size = k_cache.element_size()
     row = D * size
     if row % 16:
@@ -1094,11 +1106,11 @@ def kv_evict(k_cache: Tensor, v_cache: Tensor, scores: Tensor, block_tables: Ten
     bt, cl, nt = _rows_i32(block_tables), _i32(context_lens).contiguous(), _rows_i32(new_tables)
     lens = torch.empty(B, dtype=torch.int32, device=dev)
     kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
-    strides = (ctypes.c_longlong * 8)(*_cache_strides("key", k_cache, size, 1), *_cache_strides("value", v_cache, size, 1),
-                                      bt.stride(0), nt.stride(0))
-    _ck(_lib().tt_kv_evict(k_cache.data_ptr(), v_cache.data_ptr(), scores.data_ptr(), bt.data_ptr(), cl.data_ptr(), nt.data_ptr(),
-                           lens.data_ptr(), kept.data_ptr(), strides, B, Hkv, bs, bt.shape[1], nt.shape[1], nb, row, keep, recent,
-                           _stream_of(dev)), "tt_kv_evict")
+    args = _EVICT_ARGS.pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), scores.data_ptr(), bt.data_ptr(), cl.data_ptr(), nt.data_ptr(), lens.data_ptr(),
+        kept.data_ptr(), *_cache_strides(k_cache, v_cache, size, 1), bt.stride(0), nt.stride(0), B, Hkv, page, width, nt.shape[1], pages,
+        row, keep, recent)
+    _ck(_lib().tt_kv_evict(args, _stream_of(dev)), "tt_kv_evict")
     return lens, kept
 
 
@@ -1116,29 +1128,40 @@ def adjust_logits(logits: Tensor, tokens, lens, prompt_lens, rep, pres, freq, bi
         logits = logits.contiguous()
     if out is None:
         out = logits.new_empty((B, V))
-    # what is converted is bound to a name: it must outlive the launch
-    tok = cl = cp = ids = vals = mask = None
+    # addresses of what is there; what is converted is bound to a name, as it must outlive the launch
+    tok = cl = cp = rep_t = pres_t = freq_t = ids = vals = mask = 0
     length = entries = wide = tok_row = ids_row = vals_row = mask_row = 0
     if tokens is not None:
         length, wide = tokens.shape[1], int(tokens.dtype == torch.int64)
-        tok = tokens if length <= 1 or tokens.stride(1) == 1 else tokens.contiguous()
-        tok_row = tok.stride(0)
-        cl = None if lens is None else _i32(lens).contiguous()
-        cp = None if prompt_lens is None else _i32(prompt_lens).contiguous()
+        if length > 1 and tokens.stride(1) != 1:
+            tokens = tokens.contiguous()
+        tok, tok_row = tokens.data_ptr(), tokens.stride(0)
+        if lens is not None:
+            lens = _i32(lens).contiguous()
+            cl = lens.data_ptr()
+        if prompt_lens is not None:
+            prompt_lens = _i32(prompt_lens).contiguous()
+            cp = prompt_lens.data_ptr()
     if bias_ids is not None:
         entries = bias_ids.shape[1]
-        ids, vals = _rows_i32(bias_ids), bias_values if bias_values.stride(1) == 1 else bias_values.contiguous()
-        ids_row, vals_row = ids.stride(0), vals.stride(0)
+        bias_ids, bias_values = _rows_i32(bias_ids), bias_values if bias_values.stride(1) == 1 else bias_values.contiguous()
+        ids, vals, ids_row, vals_row = bias_ids.data_ptr(), bias_values.data_ptr(), bias_ids.stride(0), bias_values.stride(0)
     if allowed is not None:
-        mask = allowed if allowed.stride(1) == 1 else allowed.contiguous()
-        mask_row = mask.stride(0)
-    rep_t, rep = (rep.contiguous(), 0.0) if torch.is_tensor(rep) else (None, rep)
-    pres_t, pres = (pres.contiguous(), 0.0) if torch.is_tensor(pres) else (None, pres)
-    freq_t, freq = (freq.contiguous(), 0.0) if torch.is_tensor(freq) else (None, freq)
-    strides = (ctypes.c_longlong * 6)(logits.stride(0), out.stride(0), tok_row, ids_row, vals_row, mask_row)
-    _ck(_lib().tt_process_logits(logits.data_ptr(), out.data_ptr(), _p(tok), wide, _p(cl), _p(cp), _p(rep_t), _p(pres_t), _p(freq_t),
-                                 rep, pres, freq, _p(ids), _p(vals), entries, _p(mask), strides, B, V, length,
-                                 _LOGIT_TYPES[logits.dtype], _stream_of(dev)), "tt_process_logits")
+        if allowed.stride(1) != 1:
+            allowed = allowed.contiguous()
+        mask, mask_row = allowed.data_ptr(), allowed.stride(0)
+    if torch.is_tensor(rep):
+        per_row_rep, rep = rep.contiguous(), 1.0
+        rep_t = per_row_rep.data_ptr()
+    if torch.is_tensor(pres):
+        per_row_pres, pres = pres.contiguous(), 0.0
+        pres_t = per_row_pres.data_ptr()
+    if torch.is_tensor(freq):
+        per_row_freq, freq = freq.contiguous(), 0.0
+        freq_t = per_row_freq.data_ptr()
+    args = _LOGIT_ARGS.pack(logits.data_ptr(), out.data_ptr(), tok, cl, cp, rep_t, pres_t, freq_t, ids, vals, mask, logits.stride(0),
+                            out.stride(0), tok_row, ids_row, vals_row, mask_row, wide, entries, B, V, length, _LOGIT_TYPES[logits.dtype])
+    _ck(_lib().tt_process_logits(args, rep, pres, freq, _stream_of(dev)), "tt_process_logits")
     return out
 
 

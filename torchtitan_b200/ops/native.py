@@ -66,10 +66,11 @@ def lib():
         _sig(L.tt_grouped_gemm_set_pair, [I], None)
     _sig(L.tt_kv_write, [P, P, P, P, P, LL, I, I, P])
     _sig(L.tt_paged_decode, [P, P, P, P, P, P, F, I, I, I, I, I, I, P])
-    _sig(L.tt_paged_split_chunks, [I, I])
-    _sig(L.tt_paged_split, [P] * 14 + [I] * 10 + [F, I, P])
-    _sig(L.tt_kv_evict, [P] * 9 + [I] * 9 + [P])
-    _sig(L.tt_process_logits, [P, P, P, I, P, P, P, P, P, F, F, F, P, P, I, P, P, I, I, I, I, P])
+    _sig(L.tt_paged_split_least_chunk, [])
+    _sig(L.tt_paged_split_most_chunks, [])
+    _sig(L.tt_paged_split, [P, F, P])
+    _sig(L.tt_kv_evict, [P, P])
+    _sig(L.tt_process_logits, [P, F, F, F, P])
     _sig(L.tt_sample, [P, P, P, P, I, I, LL, F, I, P])
     _sig(L.tt_moe_route_fwd, [P, P, P, P, P, I, I, I, I, I, F, P])
     _sig(L.tt_moe_route_bwd, [P, P, P, P, I, I, I, I, I, F, P])

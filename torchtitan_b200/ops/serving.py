@@ -71,8 +71,10 @@ def _whole_numbers(t, name: str, rows: int, dims: int, device) -> None:
 
 
 def _no_gradient(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
 def _check_cache(k_cache, v_cache, scores, block_tables, context_lens, batch: int) -> None:
