@@ -13,6 +13,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include <atomic>
 
 namespace cg = cooperative_groups;
@@ -47,15 +49,15 @@ __device__ __forceinline__ uint32_t key_at(const Args& a, int b, int h, int t) {
   return key_of(a.scores[(static_cast<long long>(p) * a.Hkv + h) * a.page + t % a.page]);
 }
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32;
-static_assert(kWarps == 32, "block_scan keeps one warp sum per lane");
-constexpr int kBins = 2048;           // two to a thread
+constexpr int kBins = 2048;
 constexpr int kMostParts = 8;
 constexpr int kAhead = 4;
 constexpr int kMostHeld = 48 * 1024;      // keys
 
 // Exclusive sum over the block's threads; total: the sum of all.
+template <int WARPS>
 __device__ __forceinline__ int block_scan(int v, int* s_warp, int& total) {
+  static_assert(WARPS <= 32, "one warp sum per lane");
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   int inc = v;
 #pragma unroll
@@ -65,21 +67,23 @@ __device__ __forceinline__ int block_scan(int v, int* s_warp, int& total) {
   }
   if (lane == 31) s_warp[warp] = inc;
   __syncthreads();
-  const int mine = s_warp[lane];
+  const int mine = lane < WARPS ? s_warp[lane] : 0;
   int w = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
+  for (int o = 1; o < WARPS; o <<= 1) {
     const int up = __shfl_up_sync(0xffffffffu, w, o);
     if (lane >= o) w += up;
   }
-  total = __shfl_sync(0xffffffffu, w, 31);
+  total = __shfl_sync(0xffffffffu, w, WARPS - 1);
   const int before = __shfl_sync(0xffffffffu, w - mine, warp);
   __syncthreads();
   return before + inc - v;
 }
 
 // Cluster = (kv head, sequence), its CTAs cut the tokens into equal parts: writes the kept indices in order.
+template <int kThreads>
 __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
+  constexpr int kWarps = kThreads / 32, kEach = kBins / kThreads;      // bins of a thread
   asm volatile("griddepcontrol.launch_dependents;");
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), part = cluster.block_rank();
@@ -98,12 +102,13 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
   if (want == 0) return;
 
   extern __shared__ uint32_t keys[];
-  __shared__ __align__(8) int hist[2][kBins];
+  __shared__ __align__(16) int hist[2][kBins];
   __shared__ uint32_t s_lo, s_hi;
   __shared__ int s_warp[kWarps], s_want, s_bin, s_in_bin;
   __shared__ int s_above, s_equal;
   const int per = (old + parts - 1) / parts, t0 = min(old, part * per), count = min(old, t0 + per) - t0;
-  auto key = [&](int i) { return i < a.held ? keys[i] : key_at(a, b, h, t0 + i); };
+  const bool all_held = count <= a.held;
+  auto key = [&](int i) { return all_held || i < a.held ? keys[i] : key_at(a, b, h, t0 + i); };
 
   if (tid == 0) { s_lo = 0xffffffffu; s_hi = 0; }
   for (int i = tid; i < 2 * kBins; i += kThreads) hist[0][i] = 0;
@@ -154,27 +159,34 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
       if (k >= lo && k <= hi) atomicAdd(&mine[(k - lo) >> shift], 1);
     }
     meet();
-    // bins from the top, two to a thread; all parts' loads at once
-    int c[2] = {0, 0};
-    int2 of[kMostParts];
-#pragma unroll
-    for (int p = 0; p < kMostParts; ++p)
-      of[p] = p < parts ? *reinterpret_cast<const int2*>(cluster.map_shared_rank(mine, p) + kBins - 2 - 2 * tid) : make_int2(0, 0);
+    // bins from the top, kEach to a thread; all parts' loads at once
+    using Bins = std::conditional_t<kEach == 4, int4, int2>;
+    union { Bins v; int n[kEach]; } of[kMostParts];
+    int c[kEach];
 #pragma unroll
     for (int p = 0; p < kMostParts; ++p) {
-      c[0] += of[p].y;
-      c[1] += of[p].x;
+      of[p].v = Bins{};
+      if (p < parts)
+        of[p].v = *reinterpret_cast<const Bins*>((parts > 1 ? cluster.map_shared_rank(mine, p) : mine) + kBins - kEach * (tid + 1));
+    }
+    int sum = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      c[e] = 0;
+#pragma unroll
+      for (int p = 0; p < kMostParts; ++p) c[e] += of[p].n[kEach - 1 - e];
+      sum += c[e];
     }
     int total;
-    const int before = block_scan(c[0] + c[1], s_warp, total);
+    int above = block_scan<kWarps>(sum, s_warp, total);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int above = before + (e ? c[0] : 0);
+    for (int e = 0; e < kEach; ++e) {
       if (above < want && above + c[e] >= want) {
-        s_bin = kBins - 1 - 2 * tid - e;
+        s_bin = kBins - 1 - kEach * tid - e;
         s_want = want - above;
         s_in_bin = c[e];
       }
+      above += c[e];
     }
     // the histogram of the round after next; the others are done with the one of the round before this one
     for (int i = tid; i < kBins; i += kThreads) hist[(round + 1) & 1][i] = 0;
@@ -197,8 +209,8 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
   above = __reduce_add_sync(0xffffffffu, above);
   equal = __reduce_add_sync(0xffffffffu, equal);
   int all_above, all_equal;
-  int above_at = block_scan(lane == 0 ? above : 0, s_warp, all_above);
-  int equal_at = block_scan(lane == 0 ? equal : 0, s_warp, all_equal);
+  int above_at = block_scan<kWarps>(lane == 0 ? above : 0, s_warp, all_above);
+  int equal_at = block_scan<kWarps>(lane == 0 ? equal : 0, s_warp, all_equal);
   if (tid == 0) { s_above = all_above; s_equal = all_equal; }
   meet();
   for (int p = 0; p < part; ++p) {
@@ -288,11 +300,15 @@ int tt_kv_evict(const long long* v, cudaStream_t st) {
          static_cast<const int*>(at(LENS)), static_cast<const int*>(at(FRESH)), static_cast<int*>(at(NEW_LENS)),
          static_cast<int*>(at(KEPT)), v[K_PAGE], v[K_TOK], v[K_HEAD], v[V_PAGE], v[V_TOK], v[V_HEAD], v[TABLE_ROW], v[FRESH_ROW],
          B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held, page & (page - 1) ? -1 : __builtin_ctz(page)};
-  static std::atomic<uint64_t> ready{0};          // devices on which the kernel may take its shared memory
+  // many rows: blocks of 512 threads, several to an SM; few: 1024 threads each
+  const bool wide = static_cast<long long>(B) * Hkv * parts < 148;
+  const auto select = wide ? select_kernel<1024> : select_kernel<512>;
+  static std::atomic<uint64_t> ready{0};          // devices on which the kernels may take their shared memory
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -4;
   if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    if (cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostHeld * 4) != cudaSuccess) return -4;
+    for (const auto f : {select_kernel<1024>, select_kernel<512>})
+      if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostHeld * 4) != cudaSuccess) return -4;
     ready.fetch_or(uint64_t{1} << dev);
   }
   cudaLaunchAttribute attr[1];
@@ -301,12 +317,12 @@ int tt_kv_evict(const long long* v, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(Hkv * parts, B);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(wide ? 1024 : 512);
   cfg.dynamicSmemBytes = static_cast<size_t>(held) * 4;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, select_kernel, a) != cudaSuccess) return -4;
+  if (cudaLaunchKernelEx(&cfg, select, a) != cudaSuccess) return -4;
   const long long threads = (most + kRowsEach - 1) / kRowsEach * Hkv * (row_bytes / 16);
   if (threads > 0) {
     // the move's CTAs come up while the selection runs and wait there for its end
