@@ -26,7 +26,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMinChunk = 512;    // tokens
 constexpr int kMaxChunks = 256;   // per sequence: bounds the workspace and the join's work
 constexpr int kTile = 8;          // query heads of one kv head in a tile of columns
-constexpr int kMaxBatch = 2048;   // sequences of one launch (their chunk counts are kept in shared memory)
+constexpr int kMaxBatch = 1024;   // sequences of one launch (their chunk counts are kept in shared memory)
 
 struct Args {
   const void *q, *k, *v;
@@ -162,24 +162,21 @@ struct Item {
 };
 
 // items are numbered ((sequence, chunk), kv head, tile), the last fastest: neighbours read the same tokens' heads, which lie
-// next to each other in the cache.
-__device__ __forceinline__ void item_at(Item& it, const Args& a, const int* before, const uint16_t* counts, int hkts, int tiles, int i) {
-  const int bc = i / hkts, hkt = i - bc * hkts;
-  it.hk = hkt / tiles;
+// next to each other in the cache. first[b]: chunks of the sequences before b. The warp looks for the last sequence that
+// begins at or before bc, 32 candidates at a time (at most two rounds).
+__device__ __forceinline__ void item_at(Item& it, const Args& a, const int* first, int bc, int hkt, int tiles) {
+  const int lane = threadIdx.x % 32;
+  it.hk = tiles == 1 ? hkt : hkt / tiles;
   it.tile = hkt - it.hk * tiles;
-  int lo = 0, hi = (a.B - 1) / 16;                // the last 16 sequences that begin at or before bc
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (before[mid] <= bc) lo = mid; else hi = mid - 1;
-  }
-  int c = bc - before[lo], b = lo * 16;
-  while (c >= counts[b]) c -= counts[b++];
+  int b = 0;
+  if (a.B > 32) b = 32 * (__popc(__ballot_sync(0xffffffffu, lane * 32 < a.B && first[lane * 32] <= bc)) - 1);
+  b += __popc(__ballot_sync(0xffffffffu, b + lane < a.B && first[b + lane] <= bc)) - 1;
   it.b = b;
-  it.c = c;
-  it.chunks = counts[b];
+  it.c = bc - first[b];
+  it.chunks = first[b + 1] - first[b];
   it.r = range_of(a, b);
   const int len = chunk_len(it.r.n - it.r.lo);
-  it.t0 = it.r.lo + c * len;
+  it.t0 = it.r.lo + it.c * len;
   it.t1 = min(it.r.n, it.t0 + len);
 }
 
@@ -196,28 +193,23 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args
   extern __shared__ __align__(128) unsigned char smem[];
   float2* s_ml = reinterpret_cast<float2*>(smem + R::kBytes);                                // [group][NT * 8]
   float* s_x = reinterpret_cast<float*>(s_ml + kGroups * kTile * NT);                        // [group][2][part][NT * 4][lane]
-  int* before = reinterpret_cast<int*>(reinterpret_cast<char*>(s_x) + kExchange);   // [groups of 16 sequences + 1]
-  uint16_t* counts = reinterpret_cast<uint16_t*>(before + (a.B + 15) / 16 + 1);           // [B]
+  int* first = reinterpret_cast<int*>(reinterpret_cast<char*>(s_x) + kExchange);                // [B + 1]
   __shared__ int s_sum[kWarps], s_free[kWarps];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, group = warp / DP, part = warp % DP;
   const int G = a.H / a.Hkv, tiles = (G + kTile * NT - 1) / (kTile * NT), hkts = a.Hkv * tiles;
   asm volatile("griddepcontrol.launch_dependents;");       // the join's CTAs may come up, and wait for this grid's end
 
-  // the sequences' chunk counts, and how many chunks come before each 16 of them
+  // how many chunks the sequences before each one have
   {
-    const int groups = (a.B + 15) / 16, per = (groups + 32 * kWarps - 1) / (32 * kWarps);
-    const int first = min(groups, tid * per), last = min(groups, first + per);
+    constexpr int kThreads = 32 * kWarps;
+    const int per = (a.B + kThreads - 1) / kThreads, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+    int sum = 0;
 #pragma unroll 4
-    for (int b = tid; b < a.B; b += 32 * kWarps) {
+    for (int b = b0; b < b1; ++b) {
       const Range r = range_of(a, b);
       const int n = r.n - r.lo;
-      counts[b] = static_cast<uint16_t>(n > 0 ? (n + chunk_len(n) - 1) / chunk_len(n) : 0);
-    }
-    __syncthreads();
-    int sum = 0;
-    for (int g = first; g < last; ++g) {
-      before[g] = sum;
-      for (int b = g * 16; b < min(a.B, g * 16 + 16); ++b) sum += counts[b];
+      first[b] = sum;
+      sum += n > 0 ? (n + chunk_len(n) - 1) / chunk_len(n) : 0;
     }
     int inc = sum;
 #pragma unroll
@@ -229,11 +221,11 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args
     __syncthreads();
     int add = inc - sum;
     for (int w = 0; w < warp; ++w) add += s_sum[w];
-    for (int g = first; g < last; ++g) before[g] += add;
-    if (tid == 32 * kWarps - 1) before[groups] = add + sum;
+    for (int b = b0; b < b1; ++b) first[b] += add;
+    if (tid == kThreads - 1) first[a.B] = add + sum;
     __syncthreads();
   }
-  const int items = before[(a.B + 15) / 16] * hkts;
+  const int items = first[a.B] * hkts;
   const uint32_t ring = smem_u32(smem) + warp * R::kStages * R::kStageBytes;
   const T* kc = static_cast<const T*>(a.k) + part * DW;
   const T* vc = static_cast<const T*>(a.v) + part * DW;
@@ -241,6 +233,8 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args
   // ---- the loads: `head` is the item being loaded, ht its next token, page its table entry for row lane % 16
   Item head = {};
   int hi = blockIdx.x, ht = 0, page = -1, slot = 0;
+  int h_bc = hi / hkts, h_hkt = hi - h_bc * hkts;
+  const int d_bc = gridDim.x / hkts, d_hkt = gridDim.x - d_bc * hkts;      // from one item of this CTA to its next
   const T *k_head = kc, *v_head = vc;             // of the item being loaded
   auto look_up = [&]() {                          // the table entry of the step at ht, ahead of its use
     const int t = ht + (lane & 15);
@@ -250,15 +244,49 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args
     page = live ? a.tables[head.b * a.table_row + at] : -1;
     if (live && (page < 0 || page >= a.pages)) page = -2;         // named outside the cache
   };
+  // q as the right operand: column = head, consecutive k in a register. The item that the warp computes next and its q are
+  // fetched when the loads reach it, two steps before.
+  Item it = {}, next = {};
+  uint2 qn[NT][DW / 16];
+  int next_i = -1, cur = -1;                      // numbers of the items in `next` and `it`
+  const int cx = 2 * (lane & 3);                  // this thread's columns (heads): cx, cx + 1 of each tile
+  auto fetch_q = [&]() {
+    const int g0 = next.tile * kTile * NT, ng = min(kTile * NT, G - g0);
+    const T* q = static_cast<const T*>(a.q) + next.b * a.q_b + (next.hk * G + g0) * a.q_h + part * DW + cx;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int g = nt * kTile + lane / 4;
+#pragma unroll
+      for (int kk = 0; kk < DW / 16; ++kk) {
+        qn[nt][kk] = make_uint2(0, 0);
+        if (g < ng) {
+          const T* qp = q + g * a.q_h + kk * 16;
+          qn[nt][kk].x = *reinterpret_cast<const uint32_t*>(qp);
+          qn[nt][kk].y = *reinterpret_cast<const uint32_t*>(qp + 8);
+        }
+      }
+    }
+  };
   auto enter = [&]() {
-    item_at(head, a, before, counts, hkts, tiles, hi);
+    item_at(head, a, first, h_bc, h_hkt, tiles);
     ht = head.t0 + group * kRows;
     k_head = kc + head.hk * a.k_head;
     v_head = vc + head.hk * a.v_head;
+    if (cur < 0 ? next_i < 0 : hi == cur + static_cast<int>(gridDim.x)) {
+      next = head;
+      next_i = hi;
+      fetch_q();
+    }
   };
   auto settle = [&]() {                           // the first step at or after (hi, ht) that this warp has
     while (hi < items && ht >= head.t1) {
       hi += gridDim.x;
+      h_bc += d_bc;
+      h_hkt += d_hkt;
+      if (h_hkt >= hkts) {
+        h_hkt -= hkts;
+        ++h_bc;
+      }
       if (hi < items) enter();
     }
     if (hi < items) look_up();
@@ -317,33 +345,15 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args
   int stage = 0;
 
   const float c2 = a.scale * kLog2e;
-  const int cx = 2 * (lane & 3);                  // this thread's columns (heads): cx, cx + 1 of each tile
-  // q as the right operand: column = head, consecutive k in a register. The next item and its q are fetched while the current
-  // one waits for its first tokens.
-  Item it = {}, next = {};
-  uint2 qn[NT][DW / 16];
-  auto fetch = [&](int i) {
-    if (i >= items) return;
-    item_at(next, a, before, counts, hkts, tiles, i);
-    const int g0 = next.tile * kTile * NT, ng = min(kTile * NT, G - g0);
-    const T* q = static_cast<const T*>(a.q) + next.b * a.q_b + (next.hk * G + g0) * a.q_h + part * DW + cx;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int g = nt * kTile + lane / 4;
-#pragma unroll
-      for (int kk = 0; kk < DW / 16; ++kk) {
-        qn[nt][kk] = make_uint2(0, 0);
-        if (g < ng) {
-          const T* qp = q + g * a.q_h + kk * 16;
-          qn[nt][kk].x = *reinterpret_cast<const uint32_t*>(qp);
-          qn[nt][kk].y = *reinterpret_cast<const uint32_t*>(qp + 8);
-        }
-      }
-    }
-  };
   int turn = 0;                                   // of the exchange's two buffers
-  fetch(blockIdx.x);
   for (int i = blockIdx.x; i < items; i += gridDim.x) {
+    cur = i;
+    if (next_i != i) {                            // the loads passed it while an earlier item was computed
+      const int bc = i / hkts;
+      item_at(next, a, first, bc, i - bc * hkts, tiles);
+      next_i = i;
+      fetch_q();
+    }
     it = next;
     const int hk = it.hk, g0 = it.tile * kTile * NT, ng = min(kTile * NT, G - g0);
     uint2 qf[NT][DW / 16];
@@ -351,7 +361,6 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int kk = 0; kk < DW / 16; ++kk) qf[nt][kk] = qn[nt][kk];
-    bool fetched = false;
     float o[NT][DW / 16][4], m[NT][2], base[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -364,10 +373,6 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args
     }
     for (int t = it.t0 + group * kRows; t < it.t1; t += kGroups * kRows) {
       load(stage == 0 ? R::kStages - 1 : stage - 1);
-      if (!fetched) {
-        fetch(i + gridDim.x);
-        fetched = true;
-      }
       wait_group<R::kStages - 1>();
       __syncwarp();
       const uint32_t ks = ring + stage * R::kStageBytes, vs = ks + kRows * R::kRowPitch;
@@ -472,8 +477,6 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args
       __syncwarp();                               // before the stage is filled again
       stage = stage + 1 == R::kStages ? 0 : stage + 1;
     }
-
-    if (!fetched) fetch(i + gridDim.x);           // a warp without a step in this item
 
     // ---- the four groups' results, in their order
 #pragma unroll
@@ -666,7 +669,7 @@ int sm_count(int dev) {
 template <typename T, int D, int NT>
 int launch(const Args& a, int dev, cudaStream_t st) {
   const int G = a.H / a.Hkv, tiles = (G + kTile * NT - 1) / (kTile * NT);
-  const int bytes = smem_bytes<D, NT>() + ((a.B + 15) / 16 + 1) * 4 + 2 * a.B;
+  const int bytes = smem_bytes<D, NT>() + (a.B + 1) * 4;
   if (bytes > kMostSmem) return -2;
   static std::atomic<uint64_t> ready{0};        // devices on which the kernel may take its shared memory
   if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {

@@ -998,7 +998,7 @@ def paged_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tens
 
 
 PAGED_SPLIT_DIMS = (64, 128, 256)
-_PAGED_SPLIT_BATCH = 2048      # sequences of one launch
+_PAGED_SPLIT_BATCH = 1024      # sequences of one launch
 
 
 def _elsewhere(device: torch.device) -> bool:
