@@ -193,3 +193,17 @@ def test_queries_on_odd_addresses():
     wide = torch.randn(2, 4 * 65 + 1, device="cuda").to(BF16)
     q = wide[:, 1:].view(2, 4, 65)[..., :64]
     assert torch.equal(_attend(q, k, v, table, n), _attend(q.clone(), k, v, table, n))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_wider_table_changes_no_bit(D):
+    """The same sequences with tables of their own width and much wider ones: the join takes another form, the sums do not."""
+    lens = [513, 1500, 16000, 7000, 0]
+    k, v, table, n, _ = make_cache(lens, hkv=2, dim=D, page=16, dtype=BF16, device="cuda")
+    q = torch.randn(len(lens), 6, D, device="cuda").to(BF16)
+    sinks = torch.randn(6, device="cuda")
+    wide = torch.zeros(len(lens), 9000, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    for s in (None, sinks):
+        a, b = _attend(q, k, v, table, n, sinks=s, return_lse=True), _attend(q, k, v, wide, n, sinks=s, return_lse=True)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

@@ -615,6 +615,60 @@ __global__ void __launch_bounds__(kJoin) join_kernel(const Args a) {
   }
 }
 
+// The same for tables of at most 32 chunks, with the same sums in the same order (a table's width must not change a bit): a
+// warp per query head, a lane for each chunk's (maximum, sum) and for D / 32 dims.
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoin) join_few_kernel(const Args a) {
+  constexpr int S = kJoin / (D / 4), V = D / 32;
+  const int lane = threadIdx.x % 32;
+  const long long bh = static_cast<long long>(blockIdx.x) * (kJoin / 32) + threadIdx.x / 32;
+  const int b = static_cast<int>(bh / a.H), h = static_cast<int>(bh % a.H);
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (b >= a.B) return;
+  const Range r = range_of(a, b);
+  const int span = r.n - r.lo, nc = span > 0 ? (span + chunk_len(span) - 1) / chunk_len(span) : 0;
+  if (nc == 1) return;                             // written by the split kernel
+  const float2* ml = a.ws_ml + static_cast<long long>(b) * a.chunks * a.H + h;
+  const float* po = a.ws_o + (static_cast<long long>(b) * a.chunks * a.H + h) * D + lane * V;
+  const float2 mine = lane < nc ? ml[static_cast<long long>(lane) * a.H] : make_float2(-INFINITY, 0.f);
+  float top = mine.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float f = ex2(mine.x - (top == -INFINITY ? 0.f : top));
+  float sum = lane < nc ? mine.y * f : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (r.bad) sum = NAN;
+  float x[S][V] = {};
+  for (int c0 = 0; c0 < nc; c0 += S) {
+    float2 y[S][V / 2];
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v)
+        y[s][v] = c0 + s < nc ? *reinterpret_cast<const float2*>(po + static_cast<long long>(c0 + s) * a.H * D + 2 * v) : make_float2(0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const float g = __shfl_sync(0xffffffffu, f, (c0 + s) % 32);          // 0 behind the last chunk
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) {
+        x[s][2 * v] += y[s][v].x * g;
+        x[s][2 * v + 1] += y[s][v].y * g;
+      }
+    }
+  }
+  float all[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    all[v] = x[0][v];
+#pragma unroll
+    for (int s = 1; s < S; ++s) all[v] += x[s][v];
+  }
+#pragma unroll
+  for (int v = 0; v < V; v += 2) finish<T, D>(a, b, h, lane * V + v, top, sum, make_float2(all[v], all[v + 1]));
+}
+
 // CTA = (chunk, kv head, sequence): a token's weights over the query heads of its kv head, added to its score. One addition
 // per page slot and sequence, atomic only because two sequences may share a page.
 __global__ void __launch_bounds__(256) score_kernel(const Args a) {
@@ -691,7 +745,14 @@ int launch(const Args& a, int dev, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (a.chunks <= 1 && !a.scores) return cudaGetLastError() == cudaSuccess ? 0 : -4;
-  if (a.chunks > 1 && cudaLaunchKernelEx(&cfg, join_kernel<T, D>, a) != cudaSuccess) return -4;
+  // a warp per head wants at least a warp for every scheduler twice over; with fewer heads a block per head is faster (384
+  // heads of 256 dims, 10 chunks: 50 us against 52 for the whole call; 2048 heads of 128, 8 chunks: 69 against 71)
+  if (a.chunks > 32 || static_cast<long long>(a.H) * a.B < 1184) {
+    if (a.chunks > 1 && cudaLaunchKernelEx(&cfg, join_kernel<T, D>, a) != cudaSuccess) return -4;
+  } else if (a.chunks > 1) {
+    cfg.gridDim = dim3(static_cast<unsigned>((static_cast<long long>(a.H) * a.B + kJoin / 32 - 1) / (kJoin / 32)));
+    if (cudaLaunchKernelEx(&cfg, join_few_kernel<T, D>, a) != cudaSuccess) return -4;
+  }
   if (a.scores && a.chunks > 0) {
     cfg.gridDim = dim3(a.chunks, a.Hkv, a.B);
     cfg.blockDim = dim3(256);
