@@ -94,10 +94,13 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(const Args a) {
   float* s_val = reinterpret_cast<float*>(s_id + a.nb);                  // [nb]
   float* s_sum = s_val + a.nb;                                           // [nb]
   __shared__ uint32_t s_again[WORDS ? kMaxBias / 32 : 1];
-  // the logits come into L2 while the history is counted
-  if (tid == 0 && v1 - v0 >= 2 * E) {
-    const uintptr_t from = reinterpret_cast<uintptr_t>(x + v0) & ~uintptr_t{15}, to = reinterpret_cast<uintptr_t>(x + v1) & ~uintptr_t{15};
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(static_cast<uint32_t>(to - from)) : "memory");
+  // the logits and their mask come into L2 while the history is counted
+  if (tid < 2 && v1 - v0 >= 64) {
+    const uintptr_t from = tid == 0 ? reinterpret_cast<uintptr_t>(x + v0) : reinterpret_cast<uintptr_t>(a.allowed + b * a.mask_row + v0 / 32);
+    const uintptr_t to = tid == 0 ? reinterpret_cast<uintptr_t>(x + v1) : reinterpret_cast<uintptr_t>(a.allowed + b * a.mask_row + v1 / 32);
+    const uint32_t size = static_cast<uint32_t>((to & ~uintptr_t{15}) - (from & ~uintptr_t{15}));
+    if ((tid == 0 || a.allowed) && size > 0)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from & ~uintptr_t{15}), "r"(size) : "memory");
   }
   Setting set{1.f, 0.f, 0.f};
   if constexpr (WORDS) {
