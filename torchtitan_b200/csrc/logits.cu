@@ -26,6 +26,7 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kMostPart = 12288;     // logits of one CTA
 constexpr int kMaxBias = 1024;
+constexpr int kAhead = 2;             // 16-byte pieces of the history that a thread loads before it counts them
 constexpr uint32_t kCount = (1u << 20) - 1, kPrompt = 1u << 20;
 
 struct Args {
@@ -68,19 +69,23 @@ __device__ __forceinline__ void each_token(const I* tok, int n, F f) {
   const int head = min(n, static_cast<int>((16 - reinterpret_cast<uintptr_t>(tok) % 16) % 16 / sizeof(I)));
   const int vectors = (n - head) / N;
   for (int i = threadIdx.x; i < head; i += kThreads) f(tok[i], i);
-#pragma unroll 4
-  for (int v = threadIdx.x; v < vectors; v += kThreads) {
-    union { uint4 v; I t[N]; } r;
-    r.v = *reinterpret_cast<const uint4*>(tok + head + v * N);
+  for (int v0 = threadIdx.x; v0 < vectors; v0 += kAhead * kThreads) {       // loads first: counting must not hold them up
+    union { uint4 v; I t[N]; } r[kAhead];
 #pragma unroll
-    for (int e = 0; e < N; ++e) f(r.t[e], head + v * N + e);
+    for (int u = 0; u < kAhead; ++u)
+      if (v0 + u * kThreads < vectors) r[u].v = *reinterpret_cast<const uint4*>(tok + head + (v0 + u * kThreads) * N);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (v0 + u * kThreads < vectors)
+#pragma unroll
+        for (int e = 0; e < N; ++e) f(r[u].t[e], head + (v0 + u * kThreads) * N + e);
   }
   for (int i = head + vectors * N + threadIdx.x; i < n; i += kThreads) f(tok[i], i);
 }
 
 // WORDS: there are penalties or biases; otherwise only the mask is applied.
 template <typename T, bool WORDS>
-__global__ void __launch_bounds__(kThreads) adjust_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 4) adjust_kernel(const Args a) {
   constexpr int E = 16 / sizeof(T);
   const int b = blockIdx.y, tid = threadIdx.x;
   const int v0 = min(a.V, static_cast<int>(blockIdx.x) * a.part), v1 = min(a.V, v0 + a.part);
