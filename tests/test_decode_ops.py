@@ -172,6 +172,35 @@ def test_split_attention_extreme_logits(device):
         assert torch.equal(out, rows_of(v, table[0], n)[at].expand(1, 2, D))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_split_attention_many_small_weights(device, dtype):
+    """One token far ahead of very many equal ones, which together hold half of the weight: each of their weights is far below
+    what fp16 can hold next to the largest."""
+    D, n = 64, 50000
+    k, v, table, lens, _ = make_cache([n], hkv=1, dim=D, page=64, dtype=dtype, device=device)
+    q = torch.zeros(1, 2, D, device=device, dtype=dtype)
+    q[..., 0], q[:, 1, 1] = 1.0, 0.03125
+    k[table[0].long()] = 0.0
+    k[..., 0] = -10.8125                                                   # e^-10.8 = 1 / 49600
+    k[..., 1] = 0.25
+    k[table[0, 300].long(), 7] = 0.0
+    v[table[0].long()] += 3.0                                              # a mean that errors of one sign would shift
+    out, lse = serving.paged_attention_split(q, k, v, table, lens, 1.0, return_lse=True)
+    check_attention(out, attention_oracle(q, k, v, table, lens, 1.0), n, D, dtype, lse)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_split_attention_sink_of_infinity_takes_everything(device):
+    k, v, table, n, _ = make_cache([40, 1200], hkv=2, dim=64, page=16, dtype=BF16, device=device)
+    q = torch.randn(2, 4, 64, generator=_gen(1)).to(BF16).to(device)
+    sinks = torch.tensor([math.inf, 0.0, math.inf, -math.inf], device=device)
+    scores = torch.zeros(k.shape[0], 2, 16, device=device)
+    out, lse = serving.paged_attention_split(q, k, v, table, n, 0.125, sinks=sinks, scores=scores, return_lse=True)
+    assert (out[:, ::2] == 0).all() and (lse[:, ::2] == math.inf).all() and torch.isfinite(scores).all()
+    assert torch.equal(out[:, 3], serving.paged_attention_split(q, k, v, table, n, 0.125)[:, 3])
+
+
 def test_split_attention_refusals():
     k, v, table, n, _ = make_cache([20, 3], hkv=2, dim=64, page=16, dtype=BF16, device="cpu")
     q = torch.randn(2, 4, 64).to(BF16)
@@ -409,6 +438,8 @@ def test_process_logits_refusals():
     base = torch.randn(2, 80)
     with pytest.raises(ValueError):
         serving.process_logits(base[:, :40], out=base[:, 1:41])
+    with pytest.raises(ValueError, match="overlap"):
+        serving.process_logits(base[:1].expand(2, 80), out=base[:1].expand(2, 80))
     assert serving.process_logits(x[:0]).shape == (0, 40)
 
 
@@ -566,8 +597,9 @@ def test_engine_bounded_cache():
     for i, p in enumerate(PROMPTS):
         alone, _ = _generate(_engine(model, **kw), prompts=[p], n=1)
         assert alone[0] == batch[2 * i] == batch[2 * i + 1]
-    with pytest.raises(RuntimeError, match="exhausted"):
-        _generate_all(_engine_of(model, 14, **kw))
+    for blocks in (14, 7, 4):                                                   # too few to go on, to fork, to hold the prompts
+        with pytest.raises(RuntimeError, match="exhausted"):
+            _generate_all(_engine_of(model, blocks, **kw))
 
 
 def _engine_of(model, blocks, **kw):
@@ -577,10 +609,11 @@ def _engine_of(model, blocks, **kw):
 
 
 def _generate_all(engine):
+    blocks = engine.cache.alloc.available
     try:
         engine.generate(PROMPTS[:2], n_samples=1, max_tokens=30, temperature=0.0, top_p=1.0)
     finally:
-        assert engine.cache.alloc.available == 14                              # nothing is lost when the blocks run out
+        assert engine.cache.alloc.available == blocks                          # nothing is lost when the blocks run out
 
 
 def test_engine_penalties_bias_and_grammar():

@@ -207,3 +207,42 @@ def test_a_wider_table_changes_no_bit(D):
     for s in (None, sinks):
         a, b = _attend(q, k, v, table, n, sinks=s, return_lse=True), _attend(q, k, v, wide, n, sinks=s, return_lse=True)
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def _evict_by_sort(scores, table, n, keep, recent):
+    """Kept tokens from a stable descending sort; scores without NaN, all sequences longer than keep."""
+    B, page, hkv = table.shape[0], scores.shape[2], scores.shape[1]
+    x = scores[table.long()].permute(0, 2, 1, 3).reshape(B, hkv, -1)
+    age = n.long().unsqueeze(1) - torch.arange(x.shape[-1], device="cuda")
+    x = x.masked_fill((age <= recent).unsqueeze(1), float("inf")).masked_fill((age <= 0).unsqueeze(1), float("-inf"))
+    return torch.sort(x, dim=-1, descending=True, stable=True).indices[..., :keep].sort(-1).values.to(torch.int32)
+
+
+@pytest.mark.parametrize("B,hkv,n,keep,recent", [(40, 4, 60000, 1000, 100), (1, 2, 500000, 70000, 5000), (2, 3, 40001, 40000, 0), (200, 1, 300, 20, 3)])
+def test_evict_long_and_many(B, hkv, n, keep, recent):
+    """More keys to a block than its shared memory holds, clusters of several sizes, many rows."""
+    page, D = 64, 8
+    width, need = -(-n // page), -(-keep // page)
+    perm = torch.randperm(B * (width + need), device="cuda").to(torch.int32)
+    table, fresh = perm[: B * width].view(B, width), perm[B * width :].view(B, need)
+    k = torch.randn(perm.numel(), page, hkv, D, device="cuda").to(BF16)
+    v = torch.randn_like(k)
+    scores = torch.empty(perm.numel(), hkv, page, device="cuda").log_normal_(-3, 2)
+    scores *= torch.rand_like(scores) > 0.5
+    lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    want = _evict_by_sort(scores, table, lens, keep, recent)
+    new_lens, kept = serving.kv_cache_evict(k, v, scores, table, lens, fresh, keep, recent)
+    assert torch.equal(kept, want) and (new_lens == keep).all()
+    idx = want[-1, -1].long()
+    for c in (k, v):
+        assert torch.equal(rows_of(c, fresh[-1], keep)[:, -1], rows_of(c, table[-1], n)[idx, -1])
+
+
+def test_very_long_history():
+    V, L = 5000, 300_001
+    x = torch.randn(2, V, device="cuda")
+    tok = torch.randint(0, V, (2, L), device="cuda")
+    tok[:, ::3] = 17
+    y = serving.process_logits(x, tok, prompt_lens=torch.tensor([0, 100_000], device="cuda"), frequency_penalty=0.25)
+    for b, p in enumerate((0, 100_000)):
+        assert torch.equal(y[b], x[b] - 0.25 * torch.bincount(tok[b, p:], minlength=V))

@@ -18,6 +18,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <type_traits>
 
 namespace {
 
@@ -124,7 +125,7 @@ __device__ __forceinline__ void finish(const Args& a, int b, int h, int d, float
     const float f = exp2f(top - base);
     x.x *= f;
     x.y *= f;
-    sum = sum * f + exp2f(sink - base);
+    sum = sum * f + (sink == all && all != -INFINITY ? 1.f : exp2f(sink - base));
     top = all;
   }
   *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + bh * D + d) = sum == 0.f ? 0u : pack2<T>(x.x / sum, x.y / sum);
@@ -189,6 +190,7 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args a) {
   using R = Ring<D>;
   constexpr int kExchange = Exchange<D, NT>::kBytes;
+  constexpr float kLift = std::is_same_v<T, __half> ? 7.f : 0.f;
   constexpr int DW = Shape<D>::kDims, DP = Shape<D>::kParts, kWarps = Shape<D>::kWarps;
   extern __shared__ __align__(128) unsigned char smem[];
   float2* s_ml = reinterpret_cast<float2*>(smem + R::kBytes);                                // [group][NT * 8]
@@ -427,8 +429,10 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args
             if (g < ng && t + r >= it.r.first && t + r < it.t1) xt[r * G + g] = s[nt][e];
           }
         }
-        // The exponents' base is the largest logit so far, or one at most 8 below it: it is raised (and what was summed is
-        // scaled) only when a logit is over 2^8 above it, which after the first step is rare. Weights up to 2^8 lose nothing.
+        // The exponents' base is the largest logit so far, or one at most 8 below it (and for fp16 another 7 below): it is raised,
+        // and what was summed is scaled, only when a logit is over 2^8 above it, which after the first step is rare. Weights
+        // then go up to 2^15. bf16 loses nothing by that; fp16, whose steps end at 2^-24, keeps weights down to 2^-32 of the
+        // largest that way, where a base at the largest itself would round what is below 2^-25 of it to nothing.
         const float big0 = fmaxf(s[nt][0], s[nt][2]), big1 = fmaxf(s[nt][1], s[nt][3]);
         if (__any_sync(0xffffffffu, big0 > m[nt][0] + 8.f || big1 > m[nt][1] + 8.f)) {
           float f[2];
@@ -439,8 +443,8 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
             top = fmaxf(top, m[nt][e]);
-            base[nt][e] = top == -INFINITY ? 0.f : top;
-            f[e] = ex2(m[nt][e] - base[nt][e]);
+            f[e] = ex2(m[nt][e] - (top == -INFINITY ? 0.f : top));
+            base[nt][e] = top == -INFINITY ? 0.f : top - kLift;
             m[nt][e] = top;
             l[nt][e] *= f[e];
           }
@@ -487,7 +491,7 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args
         x += __shfl_xor_sync(0xffffffffu, x, 4);
         x += __shfl_xor_sync(0xffffffffu, x, 8);
         x += __shfl_xor_sync(0xffffffffu, x, 16);
-        if (lane < 4 && part == 0) s_ml[group * kTile * NT + nt * kTile + cx + e] = make_float2(m[nt][e], x);
+        if (lane < 4 && part == 0) s_ml[group * kTile * NT + nt * kTile + cx + e] = make_float2(m[nt][e] - kLift, x);
       }
     const long long row = static_cast<long long>(it.b) * a.chunks * a.H + static_cast<long long>(it.c) * a.H + hk * G + g0;
     // a warp's results go through the stage of its ring that waits to be filled

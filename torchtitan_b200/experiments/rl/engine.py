@@ -255,8 +255,10 @@ class GenerationEngine:
             prompt_blocks = []
             for i, p in enumerate(prompts):
                 nblk = (len(p) + bs - 1) // bs
-                blks = [self.cache.alloc.alloc() for _ in range(nblk)]
+                blks: list[int] = []
                 prompt_blocks.append(blks)
+                for _ in range(nblk):
+                    blks.append(self.cache.alloc.alloc())
                 toks += p
                 pos += range(len(p))
                 doc += [i] * len(p)
@@ -292,13 +294,13 @@ class GenerationEngine:
                 full = len(p) // bs if self.cache.scores is None else 0      # weights are a sequence's own: no shared blocks
                 for s in range(n_samples):
                     blks = [self.cache.alloc.share(b) for b in prompt_blocks[i][:full]]
+                    seqs.append(_Seq(prompt=i, blocks=blks, length=len(p), position=len(p), tokens=[], logprobs=[]))
                     for src in prompt_blocks[i][full:]:
                         nb = self.cache.alloc.alloc()
                         self.cache.copy_block(src, nb)
                         blks.append(nb)
-                    seqs.append(_Seq(prompt=i, blocks=blks, length=len(p), position=len(p), tokens=[], logprobs=[]))
-                for b in prompt_blocks[i]:
-                    self.cache.alloc.release(b)
+                while prompt_blocks[i]:
+                    self.cache.alloc.release(prompt_blocks[i].pop())
             first_logits = logits.repeat_interleave(n_samples, dim=0)
 
             # -- decode -------------------------------------------------------------------------------------
@@ -334,6 +336,9 @@ class GenerationEngine:
                 for b in s.blocks:
                     self.cache.alloc.release(b)
                 s.blocks = []
+            for blks in locals().get("prompt_blocks", []):      # a step above raised before the samples took over
+                for b in blks:
+                    self.cache.alloc.release(b)
             if was_training:
                 self.model.train()
 

@@ -1086,7 +1086,7 @@ def paged_split(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tenso
         lse.data_ptr() if return_lse else 0, sinks.data_ptr() if sinks is not None else 0, scores.data_ptr() if scores is not None else 0,
         o, ml, tot, x, q_b, q_h, *_cache_strides(k_cache, v_cache, 2, 2), bt.stride(0), B, H, Hkv, D, page, width, pages, win, span,
         chunks, 0 if q.dtype == torch.bfloat16 else 2)
-    _ck(_lib().tt_paged_split(args, scale, _stream_of(dev)), "tt_paged_split")
+    _ck(_lib().tt_paged_split(args, float(scale), _stream_of(dev)), "tt_paged_split")
     return (out, lse) if return_lse else out
 
 

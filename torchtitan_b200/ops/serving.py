@@ -91,8 +91,8 @@ def _check_cache(k_cache, v_cache, scores, block_tables, context_lens, batch: in
         raise ValueError(f"empty cache {list(shape)}")
     _whole_numbers(block_tables, "block_tables", batch, 2, dev)
     _whole_numbers(context_lens, "context_lens", batch, 1, dev)
-    if block_tables.shape[1] * bs >= 1 << 31:
-        raise ValueError("block_tables hold 2^31 tokens or more")
+    if block_tables.shape[1] * bs >= 1 << 30:
+        raise ValueError("block_tables hold 2^30 tokens or more")
     if scores is not None:
         if scores.dtype != torch.float32:
             raise TypeError(f"scores must be fp32, got {scores.dtype}")
@@ -121,12 +121,14 @@ def paged_attention_split(q, k_cache, v_cache, block_tables, context_lens, scale
                     several sequences share collects the weights of all of them, in no fixed order;
     ``return_lse``  also returns the log of the softmax's denominator, fp32 ``[B, H]``.
 
-    A sequence without tokens gives zeros (and a denominator of the sink alone). On CUDA a length or page number outside the
-    table or the cache gives NaN for that sequence (no score is added for a page outside); on the CPU it raises. A sequence's
-    result does not depend on the others in the batch. CUDA kernels: bf16 and fp16, head_dim 64, 128 and 256, caches with
-    contiguous heads on 16-byte boundaries (other strides are free); other types and head dims take the definition below.
-    The workspace is ``4 * B * H`` bytes per chunk and head dim, and with ``scores`` as much per token of the table's width
-    (or window): give tables no wider than the longest sequence needs. No gradient.
+    A sequence without tokens gives zeros (and a denominator of the sink alone). What unused slots of the cache hold does not
+    matter; a NaN or infinity in an attended value gives NaN. On CUDA a length or page number outside the table or the cache
+    gives NaN for that sequence, in its scores too (no score is added for a page outside); on the CPU it raises. A sequence's
+    result depends neither on the others in the batch nor on the table's width. CUDA kernels: bf16 and fp16, head_dim 64, 128
+    and 256, caches with contiguous heads on 16-byte boundaries (other strides are free); other types and head dims take the
+    definition below. The workspace is ``4 * B * H * (head_dim + 2)`` bytes per 512 tokens of the table's width (or window;
+    256 times that at most), and with ``scores`` ``4 * B * H`` per token of it: give tables no wider than the longest sequence
+    needs. No gradient.
 
     The reference reaches paged attention through vLLM (torchtitan/experiments/rl/unified/models/attention.py:62-117).
     """
@@ -305,6 +307,8 @@ def process_logits(logits, tokens=None, lens=None, prompt_lens=None, *, repetiti
     if out is not None:
         if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or out.stride(-1) != 1:
             raise ValueError("out must be like logits, with contiguous rows")
+        if B > 1 and out.stride(0) < V:
+            raise ValueError("the rows of out overlap")
         same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()
         if not same and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr():
             raise ValueError("out must be logits itself or a tensor of its own")
