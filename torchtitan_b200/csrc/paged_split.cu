@@ -424,9 +424,15 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args
         if (a.ws_x && part == 0) {
           float* xt = a.ws_x + ((static_cast<long long>(it.b) * a.Hkv + hk) * a.span + (t - it.r.lo)) * G + g0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int g = nt * kTile + cx + (e & 1), r = lane / 4 + (e >> 1) * 8;
-            if (g < ng && t + r >= it.r.first && t + r < it.t1) xt[r * G + g] = s[nt][e];
+          for (int e = 0; e < 4; e += 2) {
+            const int g = nt * kTile + cx, r = lane / 4 + (e >> 1) * 8;
+            if (g >= ng || t + r < it.r.first || t + r >= it.t1) continue;
+            if (G % 2 == 0) {
+              *reinterpret_cast<float2*>(xt + r * G + g) = make_float2(s[nt][e], s[nt][e + 1]);
+            } else {
+              xt[r * G + g] = s[nt][e];
+              if (g + 1 < ng) xt[r * G + g + 1] = s[nt][e + 1];
+            }
           }
         }
         // The exponents' base is the largest logit so far, or one at most 8 below it (and for fp16 another 7 below): it is raised,
@@ -558,23 +564,45 @@ __global__ void __launch_bounds__(32 * Shape<D>::kWarps) split_kernel(const Args
   }
 }
 
-// CTA = (query head, sequence): D / 4 threads to a chunk, 1024 / D chunks side by side; the partial sums of the rows of threads
-// are added in their order.
-constexpr int kJoin = 256;
+// CTA = (query head, sequence): a warp for every 32nd chunk, a lane for D / 32 dims; the warps' sums are added in their order.
+// Where there are fewer than 32 chunks the block has fewer warps, one for each.
+constexpr int kJoinWarps = 32;
+static_assert(kMaxChunks <= 32 * kJoinWarps, "a chunk's maximum and sum to a thread");
+
+template <int V> __device__ __forceinline__ void load_dims(float (&y)[V], const float* p) {
+  if constexpr (V == 2) {
+    const float2 u = *reinterpret_cast<const float2*>(p);
+    y[0] = u.x, y[1] = u.y;
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; v += 4) {
+      const float4 u = *reinterpret_cast<const float4*>(p + v);
+      y[v] = u.x, y[v + 1] = u.y, y[v + 2] = u.z, y[v + 3] = u.w;
+    }
+  }
+}
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoin) join_kernel(const Args a) {
-  constexpr int W = D / 4, S = kJoin / W;
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid % 32, warp = tid / 32, d = tid % W * 4, s = tid / W;
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Args a) {
+  constexpr int V = D / 32, kAhead = V == 8 ? 4 : 8;
+  const int warps = blockDim.x / 32;
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const Range r = range_of(a, b);
   const int span = r.n - r.lo, nc = span > 0 ? (span + chunk_len(span) - 1) / chunk_len(span) : 0;
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (nc == 1) return;                             // written by the split kernel
-  __shared__ float s_f[kMaxChunks], s_top[kJoin / 32], s_sum[kJoin / 32];
-  __shared__ __align__(16) float4 s_x[S][W];
+  __shared__ float s_f[kMaxChunks], s_top[kJoinWarps], s_sum[kJoinWarps];
+  __shared__ __align__(16) float s_x[kJoinWarps][D];
   const float2* ml = a.ws_ml + static_cast<long long>(b) * a.chunks * a.H + h;
-  const float* po = a.ws_o + (static_cast<long long>(b) * a.chunks * a.H + h) * D + d;
+  const float* po = a.ws_o + (static_cast<long long>(b) * a.chunks * a.H + h) * D + lane * V;
+  float y[kAhead][V];
+  auto fetch = [&](int u0) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if ((u0 + u) * warps + warp < nc) load_dims<V>(y[u], po + static_cast<long long>((u0 + u) * warps + warp) * a.H * D);
+  };
+  fetch(0);                                        // on their way while the maximum is found
   const float2 mine = tid < nc ? ml[static_cast<long long>(tid) * a.H] : make_float2(-INFINITY, 0.f);
   float top = mine.x;
 #pragma unroll
@@ -582,7 +610,8 @@ __global__ void __launch_bounds__(kJoin) join_kernel(const Args a) {
   if (lane == 0) s_top[warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kMaxChunks / 32; ++w) top = fmaxf(top, s_top[w]);
+  for (int w = 0; w < kMaxChunks / 32; ++w)
+    if (w < warps) top = fmaxf(top, s_top[w]);
   const float f = ex2(mine.x - (top == -INFINITY ? 0.f : top));
   if (tid < nc) s_f[tid] = f;
   float sum = tid < nc ? mine.y * f : 0.f;
@@ -590,42 +619,46 @@ __global__ void __launch_bounds__(kJoin) join_kernel(const Args a) {
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) s_sum[warp] = sum;
   __syncthreads();
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int c = s; c < nc; c += S) {
-    const float4 y = *reinterpret_cast<const float4*>(po + static_cast<long long>(c) * a.H * D);
-    const float g = s_f[c];
-    x.x += y.x * g;
-    x.y += y.y * g;
-    x.z += y.z * g;
-    x.w += y.w * g;
+  float x[V] = {};
+  for (int u0 = 0; u0 * warps < nc; u0 += kAhead) {
+    if (u0) fetch(u0);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if ((u0 + u) * warps + warp < nc) {
+        const float g = s_f[(u0 + u) * warps + warp];
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[v] = __fadd_rn(x[v], __fmul_rn(y[u][v], g));
+      }
   }
-  s_x[s][tid % W] = x;
+#pragma unroll
+  for (int v = 0; v < V; ++v) s_x[warp][lane * V + v] = x[v];
   __syncthreads();
-  if (s == 0) {
+  if (tid < D / 2) {
     sum = r.bad ? NAN : 0.f;
 #pragma unroll
-    for (int w = 0; w < kMaxChunks / 32; ++w) sum += s_sum[w];
-#pragma unroll
-    for (int i = 1; i < S; ++i) {
-      const float4 y = s_x[i][tid];
-      x.x += y.x;
-      x.y += y.y;
-      x.z += y.z;
-      x.w += y.w;
+    for (int w = 0; w < kMaxChunks / 32; ++w)
+      if (w < warps) sum += s_sum[w];
+    float2 all = *reinterpret_cast<const float2*>(s_x[0] + 2 * tid);
+#pragma unroll 8
+    for (int w = 1; w < warps; ++w) {
+      const float2 u = *reinterpret_cast<const float2*>(s_x[w] + 2 * tid);
+      all.x += u.x;
+      all.y += u.y;
     }
-    finish<T, D>(a, b, h, d, top, sum, make_float2(x.x, x.y));
-    finish<T, D>(a, b, h, d + 2, top, sum, make_float2(x.z, x.w));
+    finish<T, D>(a, b, h, 2 * tid, top, sum, all);
   }
 }
 
 // The same for tables of at most 32 chunks, with the same sums in the same order (a table's width must not change a bit): a
 // warp per query head, a lane for each chunk's (maximum, sum) and for D / 32 dims.
+constexpr int kFewThreads = 256;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoin) join_few_kernel(const Args a) {
-  constexpr int S = kJoin / (D / 4), V = D / 32;
+__global__ void __launch_bounds__(kFewThreads) join_few_kernel(const Args a) {
+  constexpr int V = D / 32, kAhead = 8;
+  static_assert(kJoinWarps == 32, "a chunk to each of the other form's warps");
   const int lane = threadIdx.x % 32;
-  const long long bh = static_cast<long long>(blockIdx.x) * (kJoin / 32) + threadIdx.x / 32;
+  const long long bh = static_cast<long long>(blockIdx.x) * (kFewThreads / 32) + threadIdx.x / 32;
   const int b = static_cast<int>(bh / a.H), h = static_cast<int>(bh % a.H);
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -644,30 +677,19 @@ __global__ void __launch_bounds__(kJoin) join_few_kernel(const Args a) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (r.bad) sum = NAN;
-  float x[S][V] = {};
-  for (int c0 = 0; c0 < nc; c0 += S) {
-    float2 y[S][V / 2];
+  float all[V] = {};
+  for (int c0 = 0; c0 < nc; c0 += kAhead) {
+    float y[kAhead][V];
 #pragma unroll
-    for (int s = 0; s < S; ++s)
+    for (int u = 0; u < kAhead; ++u)
+      if (c0 + u < nc) load_dims<V>(y[u], po + static_cast<long long>(c0 + u) * a.H * D);
 #pragma unroll
-      for (int v = 0; v < V / 2; ++v)
-        y[s][v] = c0 + s < nc ? *reinterpret_cast<const float2*>(po + static_cast<long long>(c0 + s) * a.H * D + 2 * v) : make_float2(0.f, 0.f);
+    for (int u = 0; u < kAhead; ++u) {
+      const float g = __shfl_sync(0xffffffffu, f, (c0 + u) % 32);
+      if (c0 + u < nc)
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const float g = __shfl_sync(0xffffffffu, f, (c0 + s) % 32);          // 0 behind the last chunk
-#pragma unroll
-      for (int v = 0; v < V / 2; ++v) {
-        x[s][2 * v] += y[s][v].x * g;
-        x[s][2 * v + 1] += y[s][v].y * g;
-      }
+        for (int v = 0; v < V; ++v) all[v] = __fadd_rn(all[v], __fmul_rn(y[u][v], g));
     }
-  }
-  float all[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    all[v] = x[0][v];
-#pragma unroll
-    for (int s = 1; s < S; ++s) all[v] += x[s][v];
   }
 #pragma unroll
   for (int v = 0; v < V; v += 2) finish<T, D>(a, b, h, lane * V + v, top, sum, make_float2(all[v], all[v + 1]));
@@ -744,7 +766,7 @@ int launch(const Args& a, int dev, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.H, a.B);
-  cfg.blockDim = dim3(kJoin);
+  cfg.blockDim = dim3(32 * (a.chunks >= kJoinWarps ? kJoinWarps : a.chunks > D / 64 ? a.chunks : D / 64));
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -754,7 +776,8 @@ int launch(const Args& a, int dev, cudaStream_t st) {
   if (a.chunks > 32 || static_cast<long long>(a.H) * a.B < 1184) {
     if (a.chunks > 1 && cudaLaunchKernelEx(&cfg, join_kernel<T, D>, a) != cudaSuccess) return -4;
   } else if (a.chunks > 1) {
-    cfg.gridDim = dim3(static_cast<unsigned>((static_cast<long long>(a.H) * a.B + kJoin / 32 - 1) / (kJoin / 32)));
+    cfg.gridDim = dim3(static_cast<unsigned>((static_cast<long long>(a.H) * a.B + kFewThreads / 32 - 1) / (kFewThreads / 32)));
+    cfg.blockDim = dim3(kFewThreads);
     if (cudaLaunchKernelEx(&cfg, join_few_kernel<T, D>, a) != cudaSuccess) return -4;
   }
   if (a.scores && a.chunks > 0) {
