@@ -14,6 +14,10 @@
 // CTAs (sharing the reading among a cluster of eight, counting in the owner's shared memory, took longer at every length up
 // to 32768: 24 rows of 50021 logits 34 us against 18, 256 rows of 151936 with 2048 tokens 104 us against 67). Then it
 // streams its part, 16 bytes to a thread, which the L2 has fetched meanwhile.
+//
+// What bounds it: each logit is read and written once. 256 rows of 151936 fp32 logits with 2048 tokens of history, 32 biases and
+// a mask: 62.6 us, 5.1 TB/s, 0.77 of the measured copy rate; with a mask and one token of history 52 us. Parts of 12288 logits, four blocks of 512
+// threads to an SM: with 6144 more of the time goes to the histories (74 us against 67), with 20480 fewer blocks overlap.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -12,6 +12,17 @@
 //
 // Rows without tokens give zeros. A page number outside the cache, or a length outside the table, gives NaN for that
 // sequence and is never followed.
+//
+// What bounds it: K and V are read once, 4 * D bytes per token and kv head, against 4 * D operations per query head: memory,
+// as long as the instructions per byte stay few. So the products go to the matrix units (eight query heads share every
+// fragment of K and V; with plain multiplications the same case took 3.8 ms instead of 0.38), tokens are copied to shared
+// memory by asynchronous 16-byte copies that run two steps ahead in every warp (24 KB a warp, 192 KB an SM on their way), and
+// nothing but the meeting at a chunk's end makes warps wait for one another. A bulk copy per row took 20 cycles a row and
+// stopped at 3.5 TB/s; copies with the address of every row looked up, at 3.6.
+// Chunks of 512 tokens: with 256 the partial results and meetings cost 128 sequences up to 8192 (16/8 heads) 375 us against
+// 353, with 1024 a ragged batch is left waiting for its last chunks (64 sequences up to 4096, 32/4 heads: 99 us against 81).
+// Measured (B200, back to back calls): 128 sequences up to 8192 tokens, 16/8 heads of 128: 385 us, 5.6 TB/s, 0.86 of the
+// measured copy rate; one of 131072, 32/8 heads: 103 us, 5.2 TB/s; 64 up to 4096, 32/4 heads, with scores: 72 us, 3.9 TB/s.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -1075,7 +1075,7 @@ def paged_split(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tenso
         rows = B * H
         n_o, n_ml = (rows * chunks * D, 2 * rows * chunks) if chunks > 1 else (0, 0)
         n_tot, n_x = (2 * rows + 2, rows * span) if scores is not None else (0, 0)
-        ws = torch.empty(n_o + n_ml + n_tot + n_x, dtype=torch.float32, device=dev)
+        ws = cl.new_empty(n_o + n_ml + n_tot + n_x)                                # words of 32 bits
         o = ws.data_ptr()
         ml = o + 4 * n_o
         if n_tot:
@@ -1104,8 +1104,7 @@ def kv_evict(k_cache: Tensor, v_cache: Tensor, scores: Tensor, block_tables: Ten
     if row % 16:
         raise ValueError(f"kv_cache_evict moves rows of multiples of 16 bytes, got head_dim {D} of {k_cache.dtype}")
     bt, cl, nt = _rows_i32(block_tables), _i32(context_lens).contiguous(), _rows_i32(new_tables)
-    lens = torch.empty(B, dtype=torch.int32, device=dev)
-    kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
+    lens, kept = cl.new_empty(B), cl.new_empty((B, Hkv, keep))
     args = _EVICT_ARGS.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), scores.data_ptr(), bt.data_ptr(), cl.data_ptr(), nt.data_ptr(), lens.data_ptr(),
         kept.data_ptr(), *_cache_strides(k_cache, v_cache, size, 1), bt.stride(0), nt.stride(0), B, Hkv, page, width, nt.shape[1], pages,
