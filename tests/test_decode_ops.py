@@ -216,7 +216,7 @@ def test_split_attention_refusals():
         ({"q": q[:1]}, ValueError), ({"k_cache": k[0]}, ValueError), ({"v_cache": v[:, :8]}, ValueError), ({"v_cache": v.float()}, TypeError),
         ({"block_tables": table.float()}, TypeError), ({"block_tables": table[:1]}, ValueError), ({"context_lens": n.short()}, TypeError),
         ({"context_lens": n.view(2, 1)}, ValueError), ({"context_lens": n + 100}, ValueError), ({"context_lens": n - 4}, ValueError),
-        ({"block_tables": table + 1000}, ValueError), ({"block_tables": table - 1000}, ValueError), ({"window": 0}, ValueError),
+        ({"block_tables": table + 1000}, ValueError), ({"block_tables": table - 1000}, ValueError), ({"window": 0}, ValueError), ({"window": 2.5}, ValueError),
         ({"sinks": torch.zeros(3)}, ValueError), ({"scores": scores.double()}, TypeError), ({"scores": scores.transpose(1, 2)}, ValueError),
         ({"scores": scores[:1]}, ValueError), ({"q": q.clone().requires_grad_()}, RuntimeError), ({"k_cache": k[:0], "v_cache": v[:0]}, ValueError),
         ({"q": q.int(), "k_cache": k.int(), "v_cache": v.int()}, TypeError),
@@ -313,7 +313,7 @@ def test_evict_refusals():
 
     call()
     for kw, err in [
-        ({"keep": 0}, ValueError), ({"recent": 33}, ValueError), ({"recent": -1}, ValueError), ({"keep": 33}, ValueError),
+        ({"keep": 0}, ValueError), ({"keep": 32.0}, ValueError), ({"recent": 33}, ValueError), ({"recent": -1}, ValueError), ({"keep": 33}, ValueError),
         ({"scores": None}, ValueError), ({"scores": s.half()}, TypeError), ({"new_tables": fresh.float()}, TypeError),
         ({"new_tables": fresh[:1]}, ValueError), ({"new_tables": fresh + 1000}, ValueError), ({"new_tables": table[:, :2]}, ValueError),
         ({"new_tables": fresh[:1].expand(2, 2)}, ValueError), ({"context_lens": n + 100}, ValueError), ({"v_cache": v[1:]}, ValueError),

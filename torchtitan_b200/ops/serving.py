@@ -123,10 +123,10 @@ def paged_attention_split(q, k_cache, v_cache, block_tables, context_lens, scale
 
     A sequence without tokens gives zeros (and a denominator of the sink alone). What unused slots of the cache hold does not
     matter; a NaN or infinity in an attended value gives NaN. On CUDA a length or page number outside the table or the cache
-    gives NaN for that sequence, in its scores too (no score is added for a page outside); on the CPU it raises. A sequence's
-    result depends neither on the others in the batch nor on the table's width. CUDA kernels: bf16 and fp16, head_dim 64, 128
-    and 256, caches with contiguous heads on 16-byte boundaries (other strides are free); other types and head dims take the
-    definition below. The workspace is ``4 * B * H * (head_dim + 2)`` bytes per 512 tokens of the table's width (or window;
+    gives NaN for that sequence, in its scores too (no score is added for a page outside); on the CPU it raises. CUDA kernels:
+    bf16 and fp16, head_dim 64, 128 and 256, caches with contiguous heads on 16-byte boundaries (other strides are free); on them
+    a sequence's result depends, to the bit, neither on the others in the batch nor on the table's width. Other types and head
+    dims take the definition below. The workspace is ``4 * B * H * (head_dim + 2)`` bytes per 512 tokens of the table's width (or window;
     256 times that at most), and with ``scores`` ``4 * B * H`` per token of it: give tables no wider than the longest sequence
     needs. No gradient.
 
@@ -144,8 +144,8 @@ def paged_attention_split(q, k_cache, v_cache, block_tables, context_lens, scale
         raise ValueError(f"q is on {q.device}, the caches are on {k_cache.device}")
     if D != kd or H % hkv:
         raise ValueError(f"{H} query heads of size {D} do not go with {hkv} kv heads of size {kd}")
-    if window is not None and window < 1:
-        raise ValueError(f"window must be at least 1, got {window}")
+    if window is not None and (not isinstance(window, int) or window < 1):
+        raise ValueError(f"window must be a whole number of at least 1, got {window}")
     if sinks is not None and (tuple(sinks.shape) != (H,) or sinks.device != q.device):
         raise ValueError(f"sinks must be one value per query head [{H}] on {q.device}")
     if q.is_cuda:
@@ -161,8 +161,11 @@ def paged_attention_split(q, k_cache, v_cache, block_tables, context_lens, scale
     pos = start.unsqueeze(1) + torch.arange(span, device=q.device)
     live = pos < lens.unsqueeze(1)                                             # [B, span]
     pos = pos.clamp(max=max(room - 1, 0))
-    page = block_tables.long().gather(1, pos // bs).masked_fill(~live, 0)
+    page = block_tables.long().gather(1, pos // bs).masked_fill(~live, 0) if room else pos
     off = pos % bs
+    wrong = (page < 0) | (page >= nb)                                          # the CPU has refused these already
+    page = page.masked_fill(wrong, 0)
+    bad = wrong.any(1) | (lens < 0) | (lens > room)
     dead = ~live.view(B, span, 1, 1)
     acc = torch.float64 if q.dtype == torch.float64 else torch.float32
     k = k_cache[page, off].to(acc).masked_fill(dead, 0.0)                     # [B, span, Hkv, D]
@@ -173,7 +176,10 @@ def paged_attention_split(q, k_cache, v_cache, block_tables, context_lens, scale
         x = torch.cat((x, sinks.to(acc).view(1, hkv, H // hkv, 1).expand(B, -1, -1, 1)), dim=-1)
     lse = torch.logsumexp(x, dim=-1, keepdim=True) if x.shape[-1] else x.new_full((B, hkv, H // hkv, 1), -math.inf)
     w = torch.exp(x[..., :span] - lse.masked_fill(lse == -math.inf, 0.0))     # nothing to attend to: zero weights
+    w = w.masked_fill(bad.view(B, 1, 1, 1), math.nan)
     out = torch.einsum("bhgn,bnhd->bhgd", w, v).reshape(B, H, D).to(q.dtype)
+    out, lse = out.masked_fill(bad.view(B, 1, 1), math.nan), lse.masked_fill(bad.view(B, 1, 1, 1), math.nan)
+    live = live & ~wrong & (lens >= 0).unsqueeze(1) & (lens <= room).unsqueeze(1)
     if scores is not None:
         at = (page.unsqueeze(1) * hkv + torch.arange(hkv, device=q.device).view(1, hkv, 1)) * bs + off.unsqueeze(1)
         scores.view(-1).index_add_(0, at.reshape(-1), w.sum(2).masked_fill(~live.unsqueeze(1), 0.0).reshape(-1).float())
@@ -202,8 +208,8 @@ def kv_cache_evict(k_cache, v_cache, scores, block_tables, context_lens, new_tab
     B = block_tables.shape[0]
     _check_cache(k_cache, v_cache, scores, block_tables, context_lens, B)
     nb, bs, hkv, D = k_cache.shape
-    if keep < 1 or not 0 <= recent <= keep:
-        raise ValueError(f"keep must be at least 1 and recent in [0, keep], got {keep} and {recent}")
+    if not isinstance(keep, int) or not isinstance(recent, int) or keep < 1 or not 0 <= recent <= keep:
+        raise ValueError(f"keep must be a whole number of at least 1 and recent one in [0, keep], got {keep} and {recent}")
     _whole_numbers(new_tables, "new_tables", B, 2, k_cache.device)
     room = block_tables.shape[1] * bs
     most = min(keep, room)
