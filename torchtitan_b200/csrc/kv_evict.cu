@@ -33,7 +33,8 @@ struct Args {
   int *new_lens, *kept;      // [B], [B, Hkv, keep]
   long long k_page, k_tok, k_head, v_page, v_tok, v_head;   // bytes
   long long table_row, fresh_row;
-  int B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held, page_shift;   // held: keys of a CTA that fit its shared memory
+  int B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held, page_shift;
+  bool fours;                // four tokens of a page lie on a 16-byte boundary of the scores   // held: keys of a CTA that fit its shared memory
 };
 
 // Larger key = kept earlier. NaN counts as the largest value, both zeros are one value.
@@ -106,12 +107,12 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
   int want = a.keep - a.recent;            // of the first `old` tokens
   if (want == 0) return;
 
-  extern __shared__ uint32_t keys[];
+  extern __shared__ __align__(16) uint32_t keys[];
   __shared__ __align__(16) int hist[2][kBins];
   __shared__ uint32_t s_lo, s_hi;
   __shared__ int s_warp[kWarps], s_want, s_bin, s_in_bin;
   __shared__ int s_above, s_equal;
-  const int per = (old + parts - 1) / parts, t0 = min(old, part * per), count = min(old, t0 + per) - t0;
+  const int per = ((old + parts - 1) / parts + 3) / 4 * 4, t0 = min(old, part * per), count = min(old, t0 + per) - t0;
   const bool all_held = count <= a.held;
   auto key = [&](int i) { return all_held || i < a.held ? keys[i] : key_at(a, b, h, t0 + i); };
 
@@ -119,28 +120,59 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
   for (int i = tid; i < 2 * kBins; i += kThreads) hist[0][i] = 0;
   __syncthreads();
   uint32_t lo = 0xffffffffu, hi = 0;
-  for (int i0 = tid; i0 < count; i0 += kAhead * kThreads) {       // several loads on their way at a time, pages first
-    int page[kAhead], slot[kAhead];
-    uint32_t k[kAhead];
+  // several loads on their way at a time, pages first; four tokens of a page with each where pages allow it
+  if (a.fours) {
+    for (int i0 = 4 * tid; i0 < count; i0 += 4 * kAhead * kThreads) {
+      int page[kAhead], slot[kAhead];
+      float4 s[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int i = i0 + u * kThreads, t = t0 + i, at = a.page_shift >= 0 ? t >> a.page_shift : t / a.page;
-      slot[u] = t - at * a.page;
-      page[u] = i < count ? a.tables[b * a.table_row + at] : -1;
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + 4 * u * kThreads, t = t0 + i, at = a.page_shift >= 0 ? t >> a.page_shift : t / a.page;
+        slot[u] = t - at * a.page;
+        page[u] = i < count ? a.tables[b * a.table_row + at] : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (page[u] >= 0 && page[u] < a.pages)
+          s[u] = *reinterpret_cast<const float4*>(a.scores + (static_cast<long long>(page[u]) * a.Hkv + h) * a.page + slot[u]);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + 4 * u * kThreads;
+        if (i >= count) continue;
+        uint4 k = make_uint4(0, 0, 0, 0);
+        if (page[u] >= 0 && page[u] < a.pages) k = make_uint4(key_of(s[u].x), key_of(s[u].y), key_of(s[u].z), key_of(s[u].w));
+        if (i < a.held) *reinterpret_cast<uint4*>(keys + i) = k;         // held is a multiple of four
+        lo = min(lo, k.x);
+        hi = max(hi, k.x);
+        if (i + 1 < count) { lo = min(lo, k.y); hi = max(hi, k.y); }
+        if (i + 2 < count) { lo = min(lo, k.z); hi = max(hi, k.z); }
+        if (i + 3 < count) { lo = min(lo, k.w); hi = max(hi, k.w); }
+      }
     }
+  } else {
+    for (int i0 = tid; i0 < count; i0 += kAhead * kThreads) {     
+      int page[kAhead], slot[kAhead];
+      uint32_t k[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const bool ok = page[u] >= 0 && page[u] < a.pages;
-      const float s = ok ? a.scores[(static_cast<long long>(page[u]) * a.Hkv + h) * a.page + slot[u]] : 0.f;
-      k[u] = ok ? key_of(s) : 0u;
-    }
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u * kThreads, t = t0 + i, at = a.page_shift >= 0 ? t >> a.page_shift : t / a.page;
+        slot[u] = t - at * a.page;
+        page[u] = i < count ? a.tables[b * a.table_row + at] : -1;
+      }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int i = i0 + u * kThreads;
-      if (i >= count) continue;
-      if (i < a.held) keys[i] = k[u];
-      lo = min(lo, k[u]);
-      hi = max(hi, k[u]);
+      for (int u = 0; u < kAhead; ++u) {
+        const bool ok = page[u] >= 0 && page[u] < a.pages;
+        const float s = ok ? a.scores[(static_cast<long long>(page[u]) * a.Hkv + h) * a.page + slot[u]] : 0.f;
+        k[u] = ok ? key_of(s) : 0u;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + u * kThreads;
+        if (i >= count) continue;
+        if (i < a.held) keys[i] = k[u];
+        lo = min(lo, k[u]);
+        hi = max(hi, k[u]);
+      }
     }
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
@@ -159,10 +191,25 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
   for (int round = 0; lo < hi; ++round) {
     int* mine = hist[round & 1];
     const int shift = max(0, 21 - __clz(hi - lo));
-    for (int i = tid; i < count; i += kThreads) {
-      const uint32_t k = key(i);
-      if (k >= lo && k <= hi) atomicAdd(&mine[(k - lo) >> shift], 1);
+    // the lowest key (tokens that were never looked at, often) is counted apart: its bin would make the threads wait in line
+    int lowest = 0;
+    auto count_key = [&](uint32_t k) {
+      if (k > lo && k <= hi) atomicAdd(&mine[(k - lo) >> shift], 1);
+      lowest += k == lo;
+    };
+    if (all_held) {
+      for (int i = 4 * tid; i < count; i += 4 * kThreads) {
+        const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
+        count_key(k.x);
+        if (i + 1 < count) count_key(k.y);
+        if (i + 2 < count) count_key(k.z);
+        if (i + 3 < count) count_key(k.w);
+      }
+    } else {
+      for (int i = tid; i < count; i += kThreads) count_key(key(i));
     }
+    lowest = __reduce_add_sync(0xffffffffu, lowest);
+    if (lane == 0 && lowest) atomicAdd(&mine[0], lowest);
     meet();
     // bins from the top, kEach to a thread; all parts' loads at once
     using Bins = std::conditional_t<kEach == 4, int4, int2>;
@@ -301,12 +348,13 @@ int tt_kv_evict(const long long* v, cudaStream_t st) {
   // CTAs of a (sequence, kv head): as many as give every SM one, but none with fewer than 2048 tokens
   int parts = 1;
   while (parts < kMostParts && static_cast<long long>(B) * Hkv * parts < 148 && room / (2 * parts) >= 2048) parts *= 2;
-  const long long per = (room + parts - 1) / parts;
+  const long long per = ((room + parts - 1) / parts + 3) / 4 * 4;
   const int held = static_cast<int>(per < kMostHeld ? per : kMostHeld);
   Args a{static_cast<char*>(at(K)), static_cast<char*>(at(V)), static_cast<float*>(at(SCORES)), static_cast<const int*>(at(TABLES)),
          static_cast<const int*>(at(LENS)), static_cast<const int*>(at(FRESH)), static_cast<int*>(at(NEW_LENS)),
          static_cast<int*>(at(KEPT)), v[K_PAGE], v[K_TOK], v[K_HEAD], v[V_PAGE], v[V_TOK], v[V_HEAD], v[TABLE_ROW], v[FRESH_ROW],
-         B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held, page & (page - 1) ? -1 : __builtin_ctz(page)};
+         B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held, page & (page - 1) ? -1 : __builtin_ctz(page),
+         page % 4 == 0 && v[SCORES] % 16 == 0};
   // many rows: blocks of 512 threads, several to an SM; few: 1024 threads each
   const bool wide = static_cast<long long>(B) * Hkv * parts < 148;
   const auto select = wide ? select_kernel<1024> : select_kernel<512>;
