@@ -44,6 +44,8 @@ __device__ __forceinline__ uint32_t key_of(float v) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
+constexpr uint32_t kZero = 0x80000000u;       // key_of(0)
+
 __device__ __forceinline__ int length_of(const Args& a, int b) {
   const int n = a.lens[b];
   return n < 0 || n > a.width * a.page ? 0 : n;
@@ -109,17 +111,25 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
 
   extern __shared__ __align__(16) uint32_t keys[];
   __shared__ __align__(16) int hist[2][kBins];
-  __shared__ uint32_t s_lo, s_hi;
+  __shared__ uint32_t s_lo, s_hi, s_pos;
   __shared__ int s_warp[kWarps], s_want, s_bin, s_in_bin;
-  __shared__ int s_above, s_equal;
+  __shared__ int s_above, s_equal, s_positive;
   const int per = ((old + parts - 1) / parts + 3) / 4 * 4, t0 = min(old, part * per), count = min(old, t0 + per) - t0;
   const bool all_held = count <= a.held;
   auto key = [&](int i) { return all_held || i < a.held ? keys[i] : key_at(a, b, h, t0 + i); };
 
-  if (tid == 0) { s_lo = 0xffffffffu; s_hi = 0; }
+  if (tid == 0) { s_lo = s_pos = 0xffffffffu; s_hi = 0; s_positive = 0; }
   for (int i = tid; i < 2 * kBins; i += kThreads) hist[0][i] = 0;
   __syncthreads();
-  uint32_t lo = 0xffffffffu, hi = 0;
+  // the lowest and highest key, and apart from them those above zero: often many tokens were never looked at, and a range that
+  // reaches down to their zero would have few of its parts where the others are
+  uint32_t lo = 0xffffffffu, hi = 0, pos = 0xffffffffu;
+  int positive = 0;
+  auto see = [&](uint32_t k) {
+    lo = min(lo, k);
+    hi = max(hi, k);
+    if (k > kZero) { pos = min(pos, k); ++positive; }
+  };
   // several loads on their way at a time, pages first; four tokens of a page with each where pages allow it
   if (a.fours) {
     for (int i0 = 4 * tid; i0 < count; i0 += 4 * kAhead * kThreads) {
@@ -142,11 +152,10 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
         uint4 k = make_uint4(0, 0, 0, 0);
         if (page[u] >= 0 && page[u] < a.pages) k = make_uint4(key_of(s[u].x), key_of(s[u].y), key_of(s[u].z), key_of(s[u].w));
         if (i < a.held) *reinterpret_cast<uint4*>(keys + i) = k;         // held is a multiple of four
-        lo = min(lo, k.x);
-        hi = max(hi, k.x);
-        if (i + 1 < count) { lo = min(lo, k.y); hi = max(hi, k.y); }
-        if (i + 2 < count) { lo = min(lo, k.z); hi = max(hi, k.z); }
-        if (i + 3 < count) { lo = min(lo, k.w); hi = max(hi, k.w); }
+        see(k.x);
+        if (i + 1 < count) see(k.y);
+        if (i + 2 < count) see(k.z);
+        if (i + 3 < count) see(k.w);
       }
     }
   } else {
@@ -170,23 +179,37 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
         const int i = i0 + u * kThreads;
         if (i >= count) continue;
         if (i < a.held) keys[i] = k[u];
-        lo = min(lo, k[u]);
-        hi = max(hi, k[u]);
+        see(k[u]);
       }
     }
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
-  if (lane == 0) { atomicMin(&s_lo, lo); atomicMax(&s_hi, hi); }
+  pos = __reduce_min_sync(0xffffffffu, pos);
+  positive = __reduce_add_sync(0xffffffffu, positive);
+  if (lane == 0) {
+    atomicMin(&s_lo, lo);
+    atomicMax(&s_hi, hi);
+    atomicMin(&s_pos, pos);
+    atomicAdd(&s_positive, positive);
+  }
   auto meet = [&]() { if (parts > 1) cluster.sync(); else __syncthreads(); };
   meet();
-  lo = 0xffffffffu, hi = 0;
+  lo = pos = 0xffffffffu, hi = 0, positive = 0;
 #pragma unroll
   for (int p = 0; p < kMostParts; ++p)
     if (p < parts) {
       lo = min(lo, *cluster.map_shared_rank(&s_lo, p));
       hi = max(hi, *cluster.map_shared_rank(&s_hi, p));
+      pos = min(pos, *cluster.map_shared_rank(&s_pos, p));
+      positive += *cluster.map_shared_rank(&s_positive, p);
     }
+  if (positive >= want) {
+    lo = pos;
+  } else {
+    want -= positive;
+    hi = kZero;
+  }
   // invariant: `want` of the keys in [lo, hi] are kept, and all above hi
   for (int round = 0; lo < hi; ++round) {
     int* mine = hist[round & 1];
