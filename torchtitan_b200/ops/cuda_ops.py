@@ -1067,7 +1067,7 @@ def paged_split(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tables: Tenso
     span = min(room, win + 15) if win else room
     least, most = _split_rule()
     chunks = min(most, -(-span // least))
-    out = q.new_empty((B, H, D))
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, H, D))       # the former takes two thirds of the time
     lse = torch.empty((B, H), dtype=torch.float32, device=dev) if return_lse else None
     o = ml = tot = x = 0
     if chunks > 1 or scores is not None:
@@ -1126,7 +1126,7 @@ def adjust_logits(logits: Tensor, tokens, lens, prompt_lens, rep, pres, freq, bi
     if logits.stride(1) != 1:
         logits = logits.contiguous()
     if out is None:
-        out = logits.new_empty((B, V))
+        out = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty((B, V))
     # addresses of what is there; what is converted is bound to a name, as it must outlive the launch
     tok = cl = cp = rep_t = pres_t = freq_t = ids = vals = mask = 0
     length = entries = wide = tok_row = ids_row = vals_row = mask_row = 0

@@ -71,10 +71,9 @@ def _whole_numbers(t, name: str, rows: int, dims: int, device) -> None:
 
 
 def _no_gradient(what: str, *tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
 def _check_cache(k_cache, v_cache, scores, block_tables, context_lens, batch: int) -> None:
@@ -89,9 +88,12 @@ def _check_cache(k_cache, v_cache, scores, block_tables, context_lens, batch: in
     nb, bs, hkv, _ = shape
     if 0 in shape:
         raise ValueError(f"empty cache {list(shape)}")
-    _whole_numbers(block_tables, "block_tables", batch, 2, dev)
-    _whole_numbers(context_lens, "context_lens", batch, 1, dev)
-    if block_tables.shape[1] * bs >= 1 << 30:
+    bt, cl = block_tables, context_lens
+    if not (type(bt) is type(cl) is torch.Tensor and bt.dtype in _WHOLE and cl.dtype in _WHOLE and bt.device == cl.device == dev
+            and bt.dim() == 2 and cl.shape == bt.shape[:1] == (batch,)):      # something may be wrong: say what
+        _whole_numbers(bt, "block_tables", batch, 2, dev)
+        _whole_numbers(cl, "context_lens", batch, 1, dev)
+    if bt.shape[1] * bs >= 1 << 30:
         raise ValueError("block_tables hold 2^30 tokens or more")
     if scores is not None:
         if scores.dtype != torch.float32:
@@ -132,7 +134,8 @@ def paged_attention_split(q, k_cache, v_cache, block_tables, context_lens, scale
 
     The reference reaches paged attention through vLLM (torchtitan/experiments/rl/unified/models/attention.py:62-117).
     """
-    _no_gradient("paged_attention_split", q, k_cache, v_cache, sinks)
+    if torch.is_grad_enabled():
+        _no_gradient("paged_attention_split", q, k_cache, v_cache, sinks)
     if q.dim() != 3:
         raise ValueError(f"q must be [batch, heads, head_dim], got {list(q.shape)}")
     B, H, D = q.shape
@@ -149,10 +152,10 @@ def paged_attention_split(q, k_cache, v_cache, block_tables, context_lens, scale
     if sinks is not None and (tuple(sinks.shape) != (H,) or sinks.device != q.device):
         raise ValueError(f"sinks must be one value per query head [{H}] on {q.device}")
     if q.is_cuda:
-        from .cuda_ops import PAGED_SPLIT_DIMS, paged_split
+        from . import cuda_ops
 
-        if q.dtype in (torch.bfloat16, torch.float16) and D in PAGED_SPLIT_DIMS:
-            return paged_split(q, k_cache, v_cache, block_tables, context_lens, scale, window, sinks, scores, return_lse)
+        if D in cuda_ops.PAGED_SPLIT_DIMS and q.dtype in (torch.bfloat16, torch.float16):
+            return cuda_ops.paged_split(q, k_cache, v_cache, block_tables, context_lens, scale, window, sinks, scores, return_lse)
         warn_once(logger, f"paged_attention_split with {q.dtype}, head_dim {D} takes the PyTorch path")
     room = block_tables.shape[1] * bs
     span = room if window is None else min(room, window)
@@ -202,7 +205,8 @@ def kv_cache_evict(k_cache, v_cache, scores, block_tables, context_lens, new_tab
 
     No counterpart in the reference, whose generator keeps every token.
     """
-    _no_gradient("kv_cache_evict", k_cache, v_cache, scores)
+    if torch.is_grad_enabled():
+        _no_gradient("kv_cache_evict", k_cache, v_cache, scores)
     if scores is None:
         raise ValueError("kv_cache_evict goes by scores")
     B = block_tables.shape[0]
@@ -281,7 +285,8 @@ def process_logits(logits, tokens=None, lens=None, prompt_lens=None, *, repetiti
 
     The reference samples through vLLM without these (torchtitan/experiments/rl/unified/actors/generator.py:251-260).
     """
-    _no_gradient("process_logits", logits, bias_values, out)
+    if torch.is_grad_enabled():
+        _no_gradient("process_logits", logits, bias_values, out)
     if logits.dim() != 2:
         raise ValueError(f"logits must be [batch, vocabulary], got {list(logits.shape)}")
     if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
