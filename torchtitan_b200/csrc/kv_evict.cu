@@ -399,8 +399,9 @@ int tt_kv_evict(const long long* v, cudaStream_t st) {
   cfg.dynamicSmemBytes = static_cast<size_t>(held) * 4;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = parts > 1;                       // a block by itself is a cluster of one
   if (cudaLaunchKernelEx(&cfg, select, a) != cudaSuccess) return -4;
+  cfg.numAttrs = 1;
   const long long threads = (most + kRowsEach - 1) / kRowsEach * Hkv * (row_bytes / 16);
   if (threads > 0) {
     // the move's CTAs come up while the selection runs and wait there for its end
