@@ -11,9 +11,9 @@
 // shares one (sequence, kv head): each holds its part of the keys in shared memory and reads the others' histograms there.
 //
 // What bounds it: the move reads and writes every kept row once and is memory-bound (32 sequences up to 8192, 8 kv heads, keep
-// 2048: 545 MB in 112 us with the selection, 4.9 TB/s, 0.74 of the measured copy rate); the selection reads 4 bytes a token and
-// is a chain of some ten meetings: 20 us there, 28 of the 61 us of 2 x 131072 tokens with 4 kv heads, whose 64 blocks do not fill
-// the GPU. Clusters of 16 would, but did not fit next to each other: 92 us.
+// 2048: 545 MB, 102 us with the selection, 86 without, 0.81 and 0.97 of the measured copy rate); the selection reads 4 bytes a
+// token and is a chain of some ten meetings: 24 of the 49 us of 2 x 131072 tokens with 4 kv heads, whose 64 blocks do not fill
+// the GPU. Clusters of 16 would, but did not fit next to each other: 92 us where clusters of 8 took 57.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
