@@ -11,16 +11,15 @@
 // shares one (sequence, kv head): each holds its part of the keys in shared memory and reads the others' histograms there.
 //
 // What bounds it: the move reads and writes every kept row once and is memory-bound (32 sequences up to 8192, 8 kv heads, keep
-// 2048: 545 MB, 102 us with the selection, 86 without, 0.81 and 0.97 of the measured copy rate); the selection reads 4 bytes a
+// 2048: 545 MB, 102 us, 0.81 of the measured copy rate; 86 us where only the latest tokens stay, without a selection); the selection reads 4 bytes a
 // token and is a chain of some ten meetings: 24 of the 49 us of 2 x 131072 tokens with 4 kv heads, whose 64 blocks do not fill
 // the GPU. Clusters of 16 would, but did not fit next to each other: 92 us where clusters of 8 took 57.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <type_traits>
-
 #include <atomic>
+#include <type_traits>
 
 namespace cg = cooperative_groups;
 
@@ -33,8 +32,9 @@ struct Args {
   int *new_lens, *kept;      // [B], [B, Hkv, keep]
   long long k_page, k_tok, k_head, v_page, v_tok, v_head;   // bytes
   long long table_row, fresh_row;
-  int B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held, page_shift;
-  bool fours;                // four tokens of a page lie on a 16-byte boundary of the scores   // held: keys of a CTA that fit its shared memory
+  int B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, page_shift;
+  int held;                  // keys of a CTA that its shared memory holds, a multiple of four
+  bool fours;                // every four tokens of a page lie on a 16-byte boundary of the scores
 };
 
 // Larger key = kept earlier. NaN counts as the largest value, both zeros are one value.
@@ -376,7 +376,7 @@ int tt_kv_evict(const long long* v, cudaStream_t st) {
   Args a{static_cast<char*>(at(K)), static_cast<char*>(at(V)), static_cast<float*>(at(SCORES)), static_cast<const int*>(at(TABLES)),
          static_cast<const int*>(at(LENS)), static_cast<const int*>(at(FRESH)), static_cast<int*>(at(NEW_LENS)),
          static_cast<int*>(at(KEPT)), v[K_PAGE], v[K_TOK], v[K_HEAD], v[V_PAGE], v[V_TOK], v[V_HEAD], v[TABLE_ROW], v[FRESH_ROW],
-         B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, held, page & (page - 1) ? -1 : __builtin_ctz(page),
+         B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, page & (page - 1) ? -1 : __builtin_ctz(page), held,
          page % 4 == 0 && v[SCORES] % 16 == 0};
   // many rows: blocks of 512 threads, several to an SM; few: 1024 threads each
   const bool wide = static_cast<long long>(B) * Hkv * parts < 148;
