@@ -534,6 +534,47 @@ def test_decode_steps_with_a_bounded_cache(device):
     assert evictions >= 6
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_arguments_that_are_parts_of_larger_tensors(device):
+    """Tables, lengths, histories, biases and masks as a server slices them from its buffers give what copies give."""
+    g = _gen(9)
+    k, v, table, n, free = make_cache([600, 33, 90], hkv=2, dim=64, page=8, dtype=FP16, device=device, spare=40)
+    q = torch.randn(3, 4, 64, generator=g).to(FP16).to(device)
+    sinks = torch.randn(4, generator=g).to(BF16).to(device)
+    wide = torch.full((3, table.shape[1] + 7), -9, dtype=torch.int32, device=device)
+    wide[:, 3 : 3 + table.shape[1]] = table
+    part, every_other = wide[:, 3 : 3 + table.shape[1]], torch.stack((n, n * 0 - 1), 1)[:, 0]
+    out = serving.paged_attention_split(q, k, v, table, n, 0.125, sinks=sinks.float(), window=500)
+    assert torch.equal(out, serving.paged_attention_split(q, k, v, part, every_other, 0.125, sinks=sinks, window=500))
+    fresh = free[:24].view(3, 8).to(device)
+    fresh_wide = torch.full((3, 20), -1, dtype=torch.int32, device=device)
+    fresh_wide[:, 1:9] = fresh
+    s = torch.rand(k.shape[0], 2, 8, generator=g).to(device)
+    results = []
+    for tables, lens, new in ((table, n, fresh), (part, every_other, fresh_wide[:, 1:9])):
+        kk, vv, ss = k.clone(), v.clone(), s.clone()
+        new_lens, kept = serving.kv_cache_evict(kk, vv, ss, tables, lens, new, 60, 10)
+        results.append((new_lens, kept, kk.view(torch.int16), vv.view(torch.int16), ss))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    V, L, N = 777, 101, 13
+    logits = torch.randn(3, V + 9, generator=g).to(device)
+    tok = torch.randint(0, V, (3, 2 * L + 6), generator=g).to(device)
+    ids, vals = torch.randint(0, V, (3, N + 4), generator=g).to(device), torch.randn(3, N + 4, generator=g).to(device)
+    mask = torch.randint(-(2**31), 2**31, (3, 40), generator=g).to(torch.int32).to(device)
+    rep, lens = torch.rand(3, 2, generator=g).to(device) + 0.5, torch.tensor([[100, 0], [0, 1], [57, 2]], device=device)
+    parts = (logits[:, 5 : 5 + V], tok[:, 3 : 3 + L], lens[:, 0], lens[:, 1], ids[:, 1 : 1 + N], vals[:, 2 : 2 + N], mask[:, 7:32], rep[:, 1])
+
+    def call(x, t, n, p, i, w, m, r):
+        return serving.process_logits(x, t, n, p, repetition_penalty=r, frequency_penalty=0.3, bias_ids=i, bias_values=w, allowed=m)
+
+    assert torch.equal(call(*parts), call(*(x.clone(memory_format=torch.contiguous_format) for x in parts)))
+    stepped = tok[:, : 2 * L : 2]                                          # tokens that do not lie next to each other
+    assert torch.equal(call(parts[0], stepped, *parts[2:]), call(parts[0], stepped.contiguous(), *parts[2:]))
+    room = torch.zeros(3, V + 3, device=device)
+    got = serving.process_logits(parts[0], parts[1], frequency_penalty=0.3, out=room[:, 1 : 1 + V])
+    assert torch.equal(got, serving.process_logits(parts[0], parts[1], frequency_penalty=0.3)) and (room[:, 0] == 0).all() and (room[:, 1 + V :] == 0).all()
+
+
 def _debug_model(dtype=FP32, device="cpu"):
     import dataclasses
 

@@ -132,7 +132,7 @@ def paged_attention_split(q, k_cache, v_cache, block_tables, context_lens, scale
     256 times that at most), and with ``scores`` ``4 * B * H`` per token of it: give tables no wider than the longest sequence
     needs. No gradient.
 
-    The reference reaches paged attention through vLLM (torchtitan/experiments/rl/unified/models/attention.py:62-117).
+    Reference counterpart: the attention of the generator, torchtitan/experiments/rl/unified/models/attention.py:62-117.
     """
     if torch.is_grad_enabled():
         _no_gradient("paged_attention_split", q, k_cache, v_cache, sinks)
@@ -283,7 +283,8 @@ def process_logits(logits, tokens=None, lens=None, prompt_lens=None, *, repetiti
     0. Token and bias ids below 0 are padding; ids of ``V`` and above raise on the CPU and are skipped on CUDA. A row whose
     mask allows nothing is ``-inf`` throughout. ``out`` may be ``logits`` itself. Returns the adjusted logits. No gradient.
 
-    The reference samples through vLLM without these (torchtitan/experiments/rl/unified/actors/generator.py:251-260).
+    No counterpart in the reference, whose generator samples by temperature and top-p
+    (torchtitan/experiments/rl/unified/actors/generator.py:251-260).
     """
     if torch.is_grad_enabled():
         _no_gradient("process_logits", logits, bias_values, out)
