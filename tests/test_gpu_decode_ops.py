@@ -253,3 +253,25 @@ def test_very_long_history():
     y = serving.process_logits(x, tok, prompt_lens=torch.tensor([0, 100_000], device="cuda"), frequency_penalty=0.25)
     for b, p in enumerate((0, 100_000)):
         assert torch.equal(y[b], x[b] - 0.25 * torch.bincount(tok[b, p:], minlength=V))
+
+
+@pytest.mark.parametrize("B", [31, 33, 300, 1025])
+def test_batches_of_every_length(B):
+    """Empty, short and many-chunk sequences mixed, batches on both sides of a warp's and a launch's number of sequences: each
+    sequence as by itself."""
+    g = torch.Generator().manual_seed(B)
+    choice = torch.tensor([0, 0, 1, 17, 511, 512, 513, 1500, 2100])
+    lens = choice[torch.randint(0, len(choice), (B,), generator=g)].tolist()
+    lens[0], lens[-1] = 0, 0
+    k, v, table, n, _ = make_cache(lens, hkv=1, dim=64, page=32, dtype=BF16, device="cuda", seed=B)
+    q = torch.randn(B, 3, 64, device="cuda").to(BF16)
+    scores = torch.zeros(k.shape[0], 1, 32, device="cuda")
+    out, lse = _attend(q, k, v, table, n, scores=scores, return_lse=True)
+    empty = torch.tensor([x == 0 for x in lens], device="cuda")
+    assert (out[empty] == 0).all() and (lse[empty] == -float("inf")).all()
+    alone = torch.zeros_like(scores)
+    for b in sorted({0, 1, B // 2, B - 2, B - 1, *torch.randint(0, B, (20,), generator=g).tolist()}):
+        one, l1 = _attend(q[b : b + 1], k, v, table[b : b + 1], n[b : b + 1], scores=alone, return_lse=True)
+        assert torch.equal(one[0], out[b]) and torch.equal(l1[0], lse[b])
+        pages = table[b, : -(-lens[b] // 32)].long()
+        assert torch.equal(alone[pages], scores[pages])
