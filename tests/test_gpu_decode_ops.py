@@ -275,3 +275,27 @@ def test_batches_of_every_length(B):
         assert torch.equal(one[0], out[b]) and torch.equal(l1[0], lse[b])
         pages = table[b, : -(-lens[b] // 32)].long()
         assert torch.equal(alone[pages], scores[pages])
+
+
+@pytest.mark.parametrize("B,hkv,D,page,dtype", [(1, 1, 8, 1, BF16), (3, 2, 512, 16, FP16), (1, 8, 128, 16, torch.float32), (150, 2, 64, 7, BF16),
+                                                (2, 3, 24, 32, torch.float32), (40, 2, 128, 16, BF16)])
+@pytest.mark.parametrize("n,keep,recent", [(40, 39, 5), (700, 200, 0), (1999, 1500, 1500), (8000, 600, 599)])
+def test_evict_small_and_large_forms(B, hkv, D, page, dtype, n, keep, recent):
+    """Caches around the sizes at which the selection and the move share a launch; rows of 16 bytes to 1 KB; lengths that differ."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    lens = (n - torch.randint(0, n - keep, (B,), generator=g, device="cuda")).to(torch.int32)        # all longer than keep
+    lens[0] = n
+    width, need = -(-n // page), -(-keep // page)
+    perm = torch.randperm(B * (width + need), generator=g, device="cuda").to(torch.int32)
+    table, fresh = perm[: B * width].view(B, width), perm[B * width :].view(B, need)
+    k = torch.randn(perm.numel(), page, hkv, D, generator=g, device="cuda").to(dtype)
+    v = torch.randn(perm.numel(), page, hkv, D, generator=g, device="cuda").to(dtype)
+    scores = torch.rand(perm.numel(), hkv, page, generator=g, device="cuda").mul_(8).floor_()          # many ties
+    want = _evict_by_sort(scores, table, lens, keep, recent)
+    k0, v0, s0 = k.clone(), v.clone(), scores.clone()
+    new_lens, kept = serving.kv_cache_evict(k, v, scores, table, lens, fresh, keep, recent)
+    assert torch.equal(kept, want) and (new_lens == keep).all()
+    j, seq, h = torch.arange(keep, device="cuda"), torch.arange(B, device="cuda").view(B, 1, 1), torch.arange(hkv, device="cuda").view(1, hkv, 1)
+    sp, so, dp, do = table[seq, want // page].long(), want.long() % page, fresh[seq, (j // page).view(1, 1, -1)].long(), (j % page).view(1, 1, -1)
+    k0[dp, do, h], v0[dp, do, h], s0[dp, h, do] = k0[sp, so, h], v0[sp, so, h], s0[sp, h, so]
+    assert torch.equal(k, k0) and torch.equal(v, v0) and torch.equal(scores, s0)

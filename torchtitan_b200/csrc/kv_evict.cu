@@ -11,8 +11,8 @@
 // shares one (sequence, kv head): each holds its part of the keys in shared memory and reads the others' histograms there.
 //
 // What bounds it: the move reads and writes every kept row once and is memory-bound (32 sequences up to 8192, 8 kv heads, keep
-// 2048: 545 MB, 102 us, 0.81 of the measured copy rate; 86 us where only the latest tokens stay, without a selection); the selection reads 4 bytes a
-// token and is a chain of some ten meetings: 24 of the 49 us of 2 x 131072 tokens with 4 kv heads, whose 64 blocks do not fill
+// 2048: 545 MB, 98 us, 0.85 of the measured copy rate; 86 us where only the latest tokens stay, without a selection); the selection reads 4 bytes a
+// token and is a chain of some ten meetings: 23 of the 48 us of 2 x 131072 tokens with 4 kv heads, whose 64 blocks do not fill
 // the GPU. Clusters of 16 would, but did not fit next to each other: 92 us where clusters of 8 took 57.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -88,17 +88,16 @@ __device__ __forceinline__ int block_scan(int v, int* s_warp, int& total) {
   return before + inc - v;
 }
 
-// Cluster = (kv head, sequence), its CTAs cut the tokens into equal parts: writes the kept indices in order.
+// Writes the kept indices of kv head h of sequence b in order. `parts` CTAs of a cluster cut the tokens into equal parts (one CTA
+// alone needs none), `part` is this one.
 template <int kThreads>
-__global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
+__device__ __forceinline__ void select_rows(const Args& a, int b, int h, int parts, int part) {
   constexpr int kWarps = kThreads / 32, kEach = kBins / kThreads;      // bins of a thread
-  asm volatile("griddepcontrol.launch_dependents;");
   cg::cluster_group cluster = cg::this_cluster();
-  const int parts = cluster.num_blocks(), part = cluster.block_rank();
-  const int h = blockIdx.x / parts, b = blockIdx.y, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int n = length_of(a, b), left = min(n, a.keep);
   int* kept = a.kept + (static_cast<long long>(b) * a.Hkv + h) * a.keep;
-  if (blockIdx.x == 0 && tid == 0) a.new_lens[b] = left;
+  if (h == 0 && part == 0 && tid == 0) a.new_lens[b] = left;
   for (int j = left + part * kThreads + tid; j < a.keep; j += parts * kThreads) kept[j] = -1;
   if (n <= a.keep) {                       // the same for the whole cluster
     for (int j = part * kThreads + tid; j < n; j += parts * kThreads) kept[j] = j;
@@ -308,8 +307,44 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
   if (parts > 1) cluster.sync();           // no CTA leaves while another may read its shared memory
 }
 
-// kRowsEach kept rows to a group of row_bytes / 16 threads, 16 bytes of each row's key and value to a thread, all loads before
-// the stores; the first thread of a group moves the scores. The rows pass once: they are marked first to leave the caches.
+// Cluster = (kv head, sequence).
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) select_kernel(const Args a) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int parts = cg::this_cluster().num_blocks();
+  select_rows<kThreads>(a, blockIdx.y, blockIdx.x / parts, parts, cg::this_cluster().block_rank());
+}
+
+// Moves piece c (16 bytes of key and of value) of the kept rows j[0..N), all loads before the stores; rows at `left` and behind
+// are none. The first piece takes the scores along.
+template <int N>
+__device__ __forceinline__ void move_pieces(const Args& a, int b, int h, const int* kept, const int (&j)[N], int left, int c) {
+  uint4 kv[N], vv[N];
+  float s[N];
+  long long dst_page[N];
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    dst_page[u] = -1;
+    if (j[u] >= left) continue;
+    const int t = kept[j[u]];
+    const int sp = a.tables[b * a.table_row + t / a.page], dp = a.fresh[b * a.fresh_row + j[u] / a.page], so = t % a.page;
+    if (sp < 0 || sp >= a.pages || dp < 0 || dp >= a.pages) continue;
+    dst_page[u] = dp;
+    kv[u] = __ldcs(reinterpret_cast<const uint4*>(a.k + sp * a.k_page + so * a.k_tok + h * a.k_head + c * 16));
+    vv[u] = __ldcs(reinterpret_cast<const uint4*>(a.v + sp * a.v_page + so * a.v_tok + h * a.v_head + c * 16));
+    if (c == 0) s[u] = a.scores[(static_cast<long long>(sp) * a.Hkv + h) * a.page + so];
+  }
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    if (dst_page[u] < 0) continue;
+    const int to = j[u] % a.page;
+    __stcs(reinterpret_cast<uint4*>(a.k + dst_page[u] * a.k_page + to * a.k_tok + h * a.k_head + c * 16), kv[u]);
+    __stcs(reinterpret_cast<uint4*>(a.v + dst_page[u] * a.v_page + to * a.v_tok + h * a.v_head + c * 16), vv[u]);
+    if (c == 0) a.scores[(dst_page[u] * a.Hkv + h) * a.page + to] = s[u];
+  }
+}
+
+// kRowsEach kept rows to a group of row_bytes / 16 threads. The rows pass once: they are marked first to leave the caches.
 // 32 sequences up to 8192, 8 kv heads, keep 2048 (545 MB): 122 us with 4 rows and plain accesses, 117 with 4 marked, 118 with 2
 // plain, 111 with 2 marked, 109 with blocks of 128 instead of 256 threads (the whole call, in a graph).
 constexpr int kRowsEach = 2, kMoveThreads = 128;
@@ -325,30 +360,29 @@ __global__ void __launch_bounds__(kMoveThreads, 12) move_kernel(const Args a) {
   const int h = static_cast<int>(r % a.Hkv);
   const long long j0 = r / a.Hkv * kRowsEach;
   if (j0 >= left) return;
-  const int* kept = a.kept + (static_cast<long long>(b) * a.Hkv + h) * a.keep;
-  uint4 kv[kRowsEach], vv[kRowsEach];
-  float s[kRowsEach];
-  long long dst_page[kRowsEach];
+  int j[kRowsEach];
 #pragma unroll
-  for (int u = 0; u < kRowsEach; ++u) {
-    const int j = static_cast<int>(j0) + u;
-    dst_page[u] = -1;
-    if (j >= left) continue;
-    const int t = kept[j];
-    const int sp = a.tables[b * a.table_row + t / a.page], dp = a.fresh[b * a.fresh_row + j / a.page], so = t % a.page;
-    if (sp < 0 || sp >= a.pages || dp < 0 || dp >= a.pages) continue;
-    dst_page[u] = dp;
-    kv[u] = __ldcs(reinterpret_cast<const uint4*>(a.k + sp * a.k_page + so * a.k_tok + h * a.k_head + c * 16));
-    vv[u] = __ldcs(reinterpret_cast<const uint4*>(a.v + sp * a.v_page + so * a.v_tok + h * a.v_head + c * 16));
-    if (c == 0) s[u] = a.scores[(static_cast<long long>(sp) * a.Hkv + h) * a.page + so];
-  }
-#pragma unroll
-  for (int u = 0; u < kRowsEach; ++u) {
-    if (dst_page[u] < 0) continue;
-    const int to = static_cast<int>((j0 + u) % a.page);
-    __stcs(reinterpret_cast<uint4*>(a.k + dst_page[u] * a.k_page + to * a.k_tok + h * a.k_head + c * 16), kv[u]);
-    __stcs(reinterpret_cast<uint4*>(a.v + dst_page[u] * a.v_page + to * a.v_tok + h * a.v_head + c * 16), vv[u]);
-    if (c == 0) a.scores[(dst_page[u] * a.Hkv + h) * a.page + to] = s[u];
+  for (int u = 0; u < kRowsEach; ++u) j[u] = static_cast<int>(j0) + u;
+  move_pieces(a, b, h, a.kept + (static_cast<long long>(b) * a.Hkv + h) * a.keep, j, left, c);
+}
+
+// Small caches in one launch, as launches are most of their time: cluster = (kv head, sequence), its first CTA selects, all move.
+// 1056 tokens, 8 kv heads, keep 1024: 17.8 us a call against 20.4 with two launches (9.3 against 8.4 in a captured graph); with 512
+// threads 10.1, with clusters of 4 14.6.
+constexpr int kSmallRoom = 8192, kSmallBytes = 128 << 10;     // tokens of a table; kept keys and values to a CTA
+
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) small_kernel(const Args a) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int movers = cluster.num_blocks(), rank = cluster.block_rank(), b = blockIdx.y, h = blockIdx.x / movers;
+  if (rank == 0) select_rows<kThreads>(a, b, h, 1, 0);
+  if (movers > 1) cluster.sync(); else __syncthreads();
+  const int left = min(length_of(a, b), a.keep), per = a.row_bytes / 16, rows = movers * kThreads / per;     // rows of a pass
+  const int at = rank * kThreads + threadIdx.x, c = at % per;
+  if (at / per >= rows) return;
+  for (int j0 = at / per; j0 < left; j0 += 2 * rows) {
+    const int j[2] = {j0, j0 + rows};
+    move_pieces(a, b, h, a.kept + (static_cast<long long>(b) * a.Hkv + h) * a.keep, j, left, c);
   }
 }
 
@@ -378,6 +412,9 @@ int tt_kv_evict(const long long* v, cudaStream_t st) {
          static_cast<int*>(at(KEPT)), v[K_PAGE], v[K_TOK], v[K_HEAD], v[V_PAGE], v[V_TOK], v[V_HEAD], v[TABLE_ROW], v[FRESH_ROW],
          B, Hkv, page, width, fresh_width, pages, row_bytes, keep, recent, page & (page - 1) ? -1 : __builtin_ctz(page), held,
          page % 4 == 0 && v[SCORES] % 16 == 0};
+  int movers = 1;
+  while (movers < 8 && static_cast<long long>(B) * Hkv * movers < 148) movers *= 2;
+  const bool small = room <= kSmallRoom && most * row_bytes * 2 <= static_cast<long long>(kSmallBytes) * movers && row_bytes <= 16 * 512;
   // many rows: blocks of 512 threads, several to an SM; few: 1024 threads each
   const bool wide = static_cast<long long>(B) * Hkv * parts < 148;
   const auto select = wide ? select_kernel<1024> : select_kernel<512>;
@@ -385,7 +422,7 @@ int tt_kv_evict(const long long* v, cudaStream_t st) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -4;
   if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-    for (const auto f : {select_kernel<1024>, select_kernel<512>})
+    for (const auto f : {select_kernel<1024>, select_kernel<512>, small_kernel<1024>, small_kernel<512>})
       if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostHeld * 4) != cudaSuccess) return -4;
     ready.fetch_or(uint64_t{1} << dev);
   }
@@ -394,6 +431,17 @@ int tt_kv_evict(const long long* v, cudaStream_t st) {
   attr[0].val.clusterDim.x = parts;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
+  if (small) {
+    attr[0].val.clusterDim.x = movers;
+    cfg.gridDim = dim3(Hkv * movers, B);
+    cfg.blockDim = dim3(movers > 1 ? 1024 : 512);          // blocks alone on their SMs, or several to one
+    cfg.dynamicSmemBytes = static_cast<size_t>((room + 3) / 4 * 4) * 4;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = movers > 1;
+    a.held = static_cast<int>((room + 3) / 4 * 4);
+    return cudaLaunchKernelEx(&cfg, movers > 1 ? small_kernel<1024> : small_kernel<512>, a) == cudaSuccess ? 0 : -4;
+  }
   cfg.gridDim = dim3(Hkv * parts, B);
   cfg.blockDim = dim3(wide ? 1024 : 512);
   cfg.dynamicSmemBytes = static_cast<size_t>(held) * 4;
