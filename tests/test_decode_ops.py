@@ -710,3 +710,72 @@ def test_engine_bounded_cache_on_the_gpu(graphs):
     assert tokens == eager and lps == eager_lps
     again, again_lps = _generate(e, presence_penalty=0.5, grammar=lambda i, s: range(100, 400))
     assert all(100 <= x < 400 for t in again for x in t)
+
+
+def test_engine_captures_with_every_write_before_the_side_stream_waits(monkeypatch):
+    """Capture under a budget on fakes of the streams: between the moment the side stream waits for the current one and the moment
+    the current one waits for it, nothing is written on the current stream (the warm-up passes would not be ordered behind it),
+    and the warm-up passes see no tokens, so that they add no weights."""
+    from contextlib import contextmanager
+
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    at, writes, warm = {"stream": "current", "open": False}, [], []
+
+    class Stream:
+        def __init__(self, name="side"):
+            self.name = name
+
+        def wait_stream(self, other):
+            at["open"] = self.name == "side"
+
+    class Graph:
+        def replay(self):
+            at["replayed"] = True
+
+    @contextmanager
+    def on(stream):
+        before, at["stream"] = at["stream"], stream.name
+        yield
+        at["stream"] = before
+
+    @contextmanager
+    def capture(graph):
+        yield
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            if at["open"] and at["stream"] == "current" and func._schema.is_mutable:
+                writes.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: Stream("current"))
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", Graph)
+    monkeypatch.setattr(torch.cuda, "graph", capture)
+    e = _engine(_debug_model(), cache_budget=16, cache_recent=4, cache_slack=6)
+    e.cudagraph = True
+    forward = e._forward
+
+    def spy(tokens, positions, meta, last_index=None):
+        if at["open"]:
+            warm.append((at["stream"], meta["context_lens"].tolist()))
+        return forward(tokens, positions, meta, last_index)
+
+    e._forward = spy
+    with Watch():
+        e.generate(PROMPTS, n_samples=1, max_tokens=3, temperature=0.0, top_p=1.0)
+    assert at["replayed"] and not writes
+    assert warm and all(stream == "side" and lens == [0] * len(PROMPTS) for stream, lens in warm)
+
+
+@pytest.mark.gpu
+def test_engine_captured_steps_add_the_weights_of_eager_ones():
+    """Every captured step is the first of its batch size and width here: the accumulated weights have the bits of eager steps."""
+    model = _debug_model(BF16, "cuda")
+    kw = {"cache_budget": 16, "cache_recent": 4, "cache_slack": 6}
+    for new in (2, 3, 8, 30):
+        captured, eager = _engine(model, cudagraph=True, **kw), _engine(model, **kw)
+        assert _generate(captured, new=new) == _generate(eager, new=new)
+        assert captured.evictions == eager.evictions and torch.equal(captured.cache.scores, eager.cache.scores)

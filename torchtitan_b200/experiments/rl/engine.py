@@ -403,10 +403,10 @@ class GenerationEngine:
         if key not in self._graphs:
             static = {"tokens": tokens.clone(), "positions": positions.clone(),
                       "meta": {k: (v.clone() if torch.is_tensor(v) else v) for k, v in meta.items()}}
-            s = torch.cuda.Stream()
-            s.wait_stream(torch.cuda.current_stream())
             if self.cache.scores is not None:
                 static["meta"]["context_lens"].zero_()      # the warm-up passes must not add weights; the real lengths follow below
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())      # after the last write to what the warm-up passes read
             with torch.cuda.stream(s):
                 for _ in range(2):                      # warm-up outside capture
                     self._forward(static["tokens"], static["positions"], static["meta"])
