@@ -457,6 +457,33 @@ def test_sampler_never_draws_a_masked_token(device, top_p):
         assert set(tok.tolist()) <= {94, 1285} and torch.isfinite(lp).all()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("temperature,top_p", [(0.0, 1.0), (1.0, 1.0), (0.7, 0.9)])
+@pytest.mark.parametrize("V", [1, 33, 3001, 50021])
+def test_sampler_of_rows_that_allow_nothing(V, temperature, top_p, dtype, device):
+    """A row whose mask leaves nothing gives token 0 and a NaN log-probability, and its neighbours what they give alone."""
+    x = torch.randn(5, V, generator=_gen(V)).to(dtype).to(device)
+    allowed = torch.full((5, -(-V // 32)), -1, dtype=torch.int32, device=device)
+    allowed[1], allowed[4] = 0, 0
+    u = torch.tensor([0.0, 0.5, 0.9, 0.3, 1.0 - 2**-24], device=device)
+    tok, lp = serving.sample_top_p(serving.process_logits(x, allowed=allowed), temperature, top_p, u)
+    some = [0, 2, 3]
+    want, want_lp = serving.sample_top_p(x[some], temperature, top_p, u[some])
+    assert tok[[1, 4]].tolist() == [0, 0] and lp[[1, 4]].isnan().all()
+    assert torch.equal(tok[some], want) and torch.equal(lp[some], want_lp)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("top_p", [1.0, 0.9])
+def test_sampler_of_rows_without_a_distribution(top_p, device):
+    """Drawing from logits with NaN or infinity in them: a token of the vocabulary, marked by its log-probability."""
+    x = torch.randn(3, 2049, generator=_gen(2)).to(device)
+    x[0, 700], x[1, 1500], x[2] = math.nan, math.inf, math.nan
+    tok, lp = serving.sample_top_p(x, 1.0, top_p, torch.tensor([0.2, 0.5, 0.99], device=device))
+    assert tok.tolist() == [0, 0, 0] and lp.isnan().all()
+
+
 # ------------------------------------------------------------------------------------------ together, as a program uses them
 @pytest.mark.parametrize("device", DEVICES)
 def test_decode_steps_with_a_bounded_cache(device):

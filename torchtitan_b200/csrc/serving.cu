@@ -249,7 +249,8 @@ sample_kernel(const T* __restrict__ logits, const float* __restrict__ uniforms, 
   __syncthreads();
 
   if (mode == 0) {
-    if (tid == 0) { tokens[row] = gidx; logprobs[row] = -__logf(raw_total); }
+    // a row without a maximum (all -inf: a mask that leaves nothing) answers token 0, its raw_total is NaN
+    if (tid == 0) { tokens[row] = gidx < V ? gidx : 0; logprobs[row] = -__logf(raw_total); }
     return;
   }
   uint32_t kmin = 0;       // keys >= kmin are in the nucleus (0 keeps everything)
@@ -294,6 +295,16 @@ sample_kernel(const T* __restrict__ logits, const float* __restrict__ uniforms, 
     __syncthreads();
   }
   const float total = s_sum[nthr - 1];
+  // Without a distribution (all -inf, NaN, +inf: a sum is NaN then) the answer is token 0, whose log-probability is NaN. It is the
+  // likeliest token where no thread below owns the draw: rounding of the prefix sums can put the target past the last of them.
+  const bool sound = isfinite(total) && isfinite(raw_total);
+  if (tid == 0) {
+    const int pick = sound ? gidx : 0;
+    tokens[row] = pick;
+    logprobs[row] = (ld<T>(x, pick) - gmax) - __logf(raw_total);
+  }
+  if (!sound) return;
+  __syncthreads();
   const float target = uniforms[row] * total;
   const float before = tid > 0 ? s_sum[tid - 1] : 0.f;
   // the owner of the crossing: before <= target < s_sum[tid]; the last non-empty thread also takes target >= total

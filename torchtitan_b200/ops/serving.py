@@ -281,7 +281,8 @@ def process_logits(logits, tokens=None, lens=None, prompt_lens=None, *, repetiti
 
     The penalties are numbers or fp32 tensors ``[B]``. ``lens`` / ``prompt_lens`` (whole numbers ``[B]``) default to ``L`` and
     0. Token and bias ids below 0 are padding; ids of ``V`` and above raise on the CPU and are skipped on CUDA. A row whose
-    mask allows nothing is ``-inf`` throughout. ``out`` may be ``logits`` itself. Returns the adjusted logits. No gradient.
+    mask allows nothing is ``-inf`` throughout (:func:`sample_top_p` marks it by a log-probability of NaN). ``out`` may be
+    ``logits`` itself. Returns the adjusted logits. No gradient.
 
     No counterpart in the reference, whose generator samples by temperature and top-p
     (torchtitan/experiments/rl/unified/actors/generator.py:251-260).
@@ -363,6 +364,8 @@ def sample_top_p(logits, temperature: float, top_p: float, uniforms):
     yields the same token on every device up to rounding at CDF boundaries. The nucleus is the set of tokens at least as
     likely as the last token needed to reach a cumulative mass of ``top_p`` from the most likely down (ties at that
     probability are all kept).
+    A row that allows nothing (``-inf`` throughout, see :func:`process_logits`) gives token 0 with a log-probability of NaN, and
+    so does one with NaN or ``+inf`` in it unless it is greedy.
     ``temperature == 0`` is greedy (lowest index on ties). Returns (tokens int64 [B], log-probabilities fp32 [B]); the log-probability is taken from the
     fp32 log-softmax of the *unscaled* logits, which is what the trainer recomputes."""
     if logits.is_cuda and native.has("tt_sample") and (top_p >= 1.0 or temperature <= 0.0 or native.has("tt_sample_top_p")):
