@@ -806,3 +806,12 @@ def test_engine_captured_steps_add_the_weights_of_eager_ones():
         captured, eager = _engine(model, cudagraph=True, **kw), _engine(model, **kw)
         assert _generate(captured, new=new) == _generate(eager, new=new)
         assert captured.evictions == eager.evictions and torch.equal(captured.cache.scores, eager.cache.scores)
+
+
+def test_whole_numbers_are_narrowed_to_values_outside():
+    from torchtitan_b200.ops import cuda_ops
+
+    far = torch.tensor([0, 7, -1, -9, 2**31 - 1, 2**31, 2**32, 2**32 + 7, -(2**32), -(2**63), 2**63 - 1])
+    assert cuda_ops._i32(far).tolist() == [0, 7, -1, -1] + [2**31 - 1] * 4 + [-1, -1, 2**31 - 1]
+    near = far[:4].to(torch.int32)
+    assert cuda_ops._i32(near) is near

@@ -299,3 +299,52 @@ def test_evict_small_and_large_forms(B, hkv, D, page, dtype, n, keep, recent):
     sp, so, dp, do = table[seq, want // page].long(), want.long() % page, fresh[seq, (j // page).view(1, 1, -1)].long(), (j % page).view(1, 1, -1)
     k0[dp, do, h], v0[dp, do, h], s0[dp, h, do] = k0[sp, so, h], v0[sp, so, h], s0[sp, h, so]
     assert torch.equal(k, k0) and torch.equal(v, v0) and torch.equal(scores, s0)
+
+
+def _past_32_bits(t, at, value):
+    t = t.long().clone()
+    t[at] = value
+    return t
+
+
+@pytest.mark.parametrize("value", [2**32, 2**32 + 1, 2**31, -(2**63), -(2**32), 2**63 - 1])
+def test_whole_numbers_past_32_bits_are_outside(value):
+    """int64 tables, lengths and ids are checked by their value, not by their lower half (which names real pages and tokens)."""
+    k, v, table, n, free = make_cache([40, 64, 33], hkv=2, dim=64, page=16, dtype=BF16, device="cuda", spare=20)
+    q = torch.randn(3, 4, 64, device="cuda").to(BF16)
+    good = _attend(q, k, v, table, n)
+    for bad_t, bad_n in ((_past_32_bits(table, (0, 1), value), n.long()), (table.long(), _past_32_bits(n, 0, value))):
+        scores = torch.zeros(k.shape[0], 2, 16, device="cuda")
+        out, lse = _attend(q, k, v, bad_t, bad_n, scores=scores, return_lse=True)
+        assert out[0].isnan().all() and lse[0].isnan().all() and torch.equal(out[1:], good[1:])
+        others = torch.ones(k.shape[0], dtype=torch.bool, device="cuda")
+        others[table[0, :3].long()] = False
+        assert torch.isfinite(scores[others]).all()
+    fresh = free[:6].view(3, 2).to("cuda")
+    scores = torch.rand(k.shape[0], 2, 16, device="cuda")
+    k0 = k.clone()
+    lens, kept = serving.kv_cache_evict(k, v, scores, table, _past_32_bits(n, 0, value), fresh, 32, 4)
+    assert lens.tolist() == [0, 32, 32] and (kept[0] == -1).all()
+    assert torch.equal(k[fresh[0].long()].view(torch.int16), k0[fresh[0].long()].view(torch.int16))
+    k1 = k.clone()
+    serving.kv_cache_evict(k, v, scores, table, n, _past_32_bits(fresh, (0, 0), value), 32, 4)
+    moved = torch.zeros(k.shape[0], dtype=torch.bool, device="cuda")
+    moved[fresh.view(-1)[1:].long()] = True
+    assert torch.equal(k[~moved].view(torch.int16), k1[~moved].view(torch.int16))
+    x = torch.randn(2, 100, device="cuda")
+    tok = torch.tensor([[5, value, 6], [7, 7, value]], device="cuda")
+    far = torch.tensor([3, value], device="cuda")
+    y = serving.process_logits(x, tok, far, presence_penalty=2.0, bias_ids=torch.tensor([[value, 3], [4, value]], device="cuda"),
+                               bias_values=torch.ones(2, 2, device="cuda"))
+    want = x.clone()
+    want[0, [5, 6]] -= 2.0
+    want[1, 7] -= 2.0 if value > 0 else 0.0                                # a length above the list's is the list's, one below 0 is 0
+    want[0, 3] += 1.0
+    want[1, 4] += 1.0
+    assert torch.equal(y, want)
+    y = serving.process_logits(x, tok, prompt_lens=far * 0 + value, frequency_penalty=0.5)
+    want = x.clone()
+    if value < 0:
+        want[0, [5, 6]] -= 0.5
+        want[1, 7] -= 1.0
+    assert torch.equal(y, want)

@@ -1011,7 +1011,9 @@ def _stream_of(device: torch.device) -> int:
 
 
 def _i32(t: Tensor) -> Tensor:
-    return t if t.dtype == torch.int32 else t.to(torch.int32)
+    """``t`` in 32 bits; what does not fit becomes -1 or 2^31 - 1, which the kernels' checks see as outside (the lower half of
+    the number would name a page or token that exists)."""
+    return t if t.dtype == torch.int32 else t.clamp(-1, 2**31 - 1).to(torch.int32)
 
 
 def _rows_i32(t: Tensor) -> Tensor:
