@@ -815,3 +815,21 @@ def test_whole_numbers_are_narrowed_to_values_outside():
     assert cuda_ops._i32(far).tolist() == [0, 7, -1, -1] + [2**31 - 1] * 4 + [-1, -1, 2**31 - 1]
     near = far[:4].to(torch.int32)
     assert cuda_ops._i32(near) is near
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("beyond", [-7, 1 << 30, -(1 << 31)])
+def test_evict_does_not_look_at_table_entries_behind_a_sequence(beyond, device):
+    """Behind a sequence's pages a table may hold anything, as for the attention."""
+    k, v, table, n, free = make_cache([40, 9, 0], hkv=2, dim=64, page=16, dtype=BF16, device=device, spare=12)
+    fresh = free[:6].view(3, 2).to(device)
+    s = torch.rand(k.shape[0], 2, 16, generator=_gen(4)).to(device)
+    results = []
+    for fill in (0, beyond):
+        wide = torch.full((3, 6), fill, dtype=torch.int32, device=device)
+        for b, pages in enumerate((3, 1, 0)):
+            wide[b, :pages] = table[b, :pages]
+        kk, vv, ss = k.clone(), v.clone(), s.clone()
+        lens, kept = serving.kv_cache_evict(kk, vv, ss, wide, n, fresh, 20, 4)
+        results.append((lens, kept, kk.view(torch.int16), vv.view(torch.int16), ss))
+    assert results[0][0].tolist() == [20, 9, 0] and all(torch.equal(a, b) for a, b in zip(*results))

@@ -239,7 +239,7 @@ def kv_cache_evict(k_cache, v_cache, scores, block_tables, context_lens, new_tab
             idx = torch.arange(n)
             if n > keep:
                 first = n - recent
-                s = scores[old[b], h].reshape(-1)[:first]
+                s = scores[old[b, : -(-n // bs)], h].reshape(-1)[:first]       # behind its pages a table may hold anything
                 best = torch.sort(s, descending=True, stable=True).indices[: keep - recent]
                 idx = torch.cat((best.sort().values, torch.arange(first, n)))
             j = torch.arange(idx.numel())
