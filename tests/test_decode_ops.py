@@ -833,3 +833,15 @@ def test_evict_does_not_look_at_table_entries_behind_a_sequence(beyond, device):
         lens, kept = serving.kv_cache_evict(kk, vv, ss, wide, n, fresh, 20, 4)
         results.append((lens, kept, kk.view(torch.int16), vv.view(torch.int16), ss))
     assert results[0][0].tolist() == [20, 9, 0] and all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_evict_refuses_a_keep_past_31_bits(device):
+    """Kept tokens are counted in 32 bits: 2^32 + 5 must not become 5 (an empty batch, as `kept` has `keep` columns)."""
+    k, v, table, n, free = make_cache([40], hkv=2, dim=64, page=16, dtype=BF16, device=device, spare=8)
+    s, fresh = torch.zeros(k.shape[0], 2, 16, device=device), free[:4].view(1, 4).to(device)
+    for keep in (1 << 31, (1 << 32) + 5):
+        with pytest.raises(ValueError, match="keep"):
+            serving.kv_cache_evict(k, v, s, table[:0], n[:0], fresh[:0], keep)
+    lens, kept = serving.kv_cache_evict(k, v, s, table[:0], n[:0], fresh[:0], (1 << 31) - 1)
+    assert lens.shape == (0,) and kept.shape == (0, 2, (1 << 31) - 1)
