@@ -845,3 +845,13 @@ def test_evict_refuses_a_keep_past_31_bits(device):
             serving.kv_cache_evict(k, v, s, table[:0], n[:0], fresh[:0], keep)
     lens, kept = serving.kv_cache_evict(k, v, s, table[:0], n[:0], fresh[:0], (1 << 31) - 1)
     assert lens.shape == (0,) and kept.shape == (0, 2, (1 << 31) - 1)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sampler_draws_no_masked_token_where_rounding_keeps_everything(device):
+    """top_p next to 1: the mass of all tokens falls short of it by rounding, so that the nucleus takes the masked ones in."""
+    x = torch.stack([torch.randn(3001, generator=_gen(seed)) for seed in range(200)]).to(device)
+    x[:, 2000:] = -math.inf
+    for u in (0.5, 1.0 - 2**-24, 1.0):
+        tok, lp = serving.sample_top_p(x, 1.0, 1.0 - 2**-24, torch.full((200,), u, device=device))
+        assert int(tok.max()) < 2000 and torch.isfinite(lp).all()

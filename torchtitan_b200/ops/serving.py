@@ -388,7 +388,8 @@ def sample_top_p(logits, temperature: float, top_p: float, uniforms):
     cdf = (probs * keep).cumsum(-1)
     target = uniforms.float().view(-1, 1) * cdf[:, -1:]
     tok = (cdf <= target).sum(-1)
-    last_kept = logits.shape[-1] - 1 - keep.flip(-1).float().argmax(-1)
+    # a nucleus that rounding extends to everything holds tokens without mass too: none of them is drawn
+    last_kept = logits.shape[-1] - 1 - (keep & (probs > 0)).flip(-1).float().argmax(-1)
     tok = torch.minimum(tok, last_kept)
     return tok, logp_raw.gather(1, tok.view(-1, 1)).squeeze(1)
 
