@@ -855,3 +855,24 @@ def test_sampler_draws_no_masked_token_where_rounding_keeps_everything(device):
     for u in (0.5, 1.0 - 2**-24, 1.0):
         tok, lp = serving.sample_top_p(x, 1.0, 1.0 - 2**-24, torch.full((200,), u, device=device))
         assert int(tok.max()) < 2000 and torch.isfinite(lp).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_engine_refuses_a_step_that_leaves_no_token(temperature, device):
+    """A grammar whose only tokens a bias of -inf takes away, at the first token or a later one of one sequence."""
+    model = _debug_model(BF16 if device == "cuda" else FP32, device)
+    for at in (0, 2):
+        with pytest.raises(ValueError, match="sequence 3"):
+            _generate_then_count(_engine(model), temperature, grammar=lambda i, said, at=at: [5, 6] if i == 3 and len(said) == at else None,
+                                 logit_bias={5: -math.inf, 6: -math.inf})
+    tokens, _ = _generate(_engine(model), new=5, grammar=lambda i, said: [5, 6, 7], logit_bias={5: -math.inf, 6: -math.inf})
+    assert all(set(t) == {7} for t in tokens)
+
+
+def _generate_then_count(engine, temperature, **kw):
+    free = engine.cache.alloc.available
+    try:
+        engine.generate(PROMPTS, n_samples=2, max_tokens=4, temperature=temperature, top_p=1.0, **kw)
+    finally:
+        assert engine.cache.alloc.available == free

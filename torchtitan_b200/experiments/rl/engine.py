@@ -156,6 +156,14 @@ class _LogitShaper:
         w = (bits.view(len(rows), words, 32).long() << torch.arange(32)).sum(-1)
         return torch.where(w >= 1 << 31, w - (1 << 32), w).to(torch.int32).to(self.device)
 
+    def check(self, shaped, logprobs, active: list[int]) -> None:
+        """Refuses a step in which the grammar and the biases left a sequence nothing: the sampler marks it with NaN."""
+        if self.grammar is None and self.bias is None:
+            return
+        for j in logprobs.isnan().nonzero().flatten().tolist():
+            if bool((shaped[j] == float("-inf")).all()):
+                raise ValueError(f"the grammar and logit_bias leave sequence {active[j]} no token")
+
     def said(self, active: list[int], tokens) -> None:
         if self.penalised:
             rows = torch.tensor(active, device=self.device)
@@ -243,7 +251,7 @@ class GenerationEngine:
 
         The penalties and ``logit_bias`` (token -> added to its logit) are those of ``serving.process_logits``.
         ``grammar(i, tokens)`` is asked before every token of sequence ``i`` with what it has generated: the token ids that
-        may come next (at least one), or None for any."""
+        may come next (at least one that ``logit_bias`` leaves), or None for any."""
         dev, bs = self.device, self.block_size
         shaper = _LogitShaper(prompts, n_samples, max_tokens, repetition_penalty, presence_penalty, frequency_penalty, logit_bias,
                               grammar, dev)
@@ -312,6 +320,7 @@ class GenerationEngine:
                 shaped = shaper(cur_logits, seqs, active)
                 tok, lp = serving.sample_top_p(shaped, temperature, top_p, u)
                 if shaped is not cur_logits:
+                    shaper.check(shaped, lp, active)
                     lp = ops.token_logprobs(cur_logits, tok)
                     shaper.said(active, tok)
                 tok_l, lp_l = tok.tolist(), lp.tolist()
