@@ -876,3 +876,20 @@ def _generate_then_count(engine, temperature, **kw):
         engine.generate(PROMPTS, n_samples=2, max_tokens=4, temperature=temperature, top_p=1.0, **kw)
     finally:
         assert engine.cache.alloc.available == free
+
+
+LONG_PROMPT = [(7 * i) % 500 + 1 for i in range(90)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_engine_bounded_cache_needs_no_copy_of_a_long_prompt_per_sample(device):
+    """Prompts that outgrow the budget: the samples need their prompt's blocks once and the budget's each, and give what they
+    give with blocks to spare. 90 + 5 tokens in blocks of 4: 23 + 2 blocks (and one for padding); a sample keeps 16 + 6 tokens."""
+    model = _debug_model(BF16 if device == "cuda" else FP32, device)
+    kw = {"cache_budget": 16, "cache_recent": 4, "cache_slack": 6}
+
+    def run(num_blocks):
+        e = _engine_of(model, num_blocks, **kw)
+        return _generate(e, prompts=[LONG_PROMPT, LONG_PROMPT[:5]], n=6, new=12, temperature=1.0), e.evictions
+
+    assert run(25 + 12 * 6 + 1) == run(600)

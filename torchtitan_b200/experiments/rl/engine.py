@@ -15,9 +15,10 @@ once in a CUDA graph and replayed (inputs live in static buffers), removing per-
 For long generations, ``split_decode=True`` decodes with attention split over the cache's length, and ``cache_budget``
 bounds the tokens that a sequence keeps in the cache: attention weights are accumulated per cached token, and a sequence
 that outgrows the budget by ``cache_slack`` is cut back to its most attended tokens (per layer and kv head). Positions go on
-counting; the sequence's pages are its own, not shared with the prompt's other samples. Both keep a sequence's result
-independent of the batch it runs in. Penalties, biases and a grammar change what is drawn; the reported log-probabilities
-stay those of the model's own logits, which is what the trainer recomputes.
+counting; the sequence's pages are its own, shared with the prompt's other samples only until the first step cuts a prompt
+that outgrows the budget back. Both keep a sequence's result independent of the batch it runs in. Penalties, biases and a
+grammar change what is drawn; the reported log-probabilities stay those of the model's own logits, which is what the trainer
+recomputes.
 """
 
 from __future__ import annotations
@@ -299,7 +300,9 @@ class GenerationEngine:
             # -- fork samples: share full prompt blocks, copy the partial tail ----------------------------
             seqs: list[_Seq] = []
             for i, p in enumerate(prompts):
-                full = len(p) // bs if self.cache.scores is None else 0      # weights are a sequence's own: no shared blocks
+                # weights are a sequence's own: no shared blocks, but for those of a prompt that the first decode step cuts back
+                # into every sample's own before anything is written
+                full = len(p) // bs if self.cache.scores is None else len(prompt_blocks[i]) if self._outgrown(len(p)) else 0
                 for s in range(n_samples):
                     blks = [self.cache.alloc.share(b) for b in prompt_blocks[i][:full]]
                     seqs.append(_Seq(prompt=i, blocks=blks, length=len(p), position=len(p), tokens=[], logprobs=[]))
@@ -351,6 +354,9 @@ class GenerationEngine:
             if was_training:
                 self.model.train()
 
+    def _outgrown(self, length: int) -> bool:
+        return self.cache_budget is not None and length >= self.cache_budget + self.cache_slack
+
     def _evict(self, seqs: list[_Seq]) -> None:
         """Cut the caches of ``seqs`` back to the budget, layer by layer, into new blocks; the old ones are released."""
         if not seqs:
@@ -385,8 +391,7 @@ class GenerationEngine:
         dev, bs = self.device, self.block_size
         B = len(active)
         slots, ctx, pos, handed_out = [], [], [], []
-        if self.cache_budget is not None:
-            self._evict([seqs[si] for si in active if seqs[si].length >= self.cache_budget + self.cache_slack])
+        self._evict([seqs[si] for si in active if self._outgrown(seqs[si].length)])
         for si in active:
             s = seqs[si]
             if s.length % bs == 0 and s.length // bs >= len(s.blocks):
