@@ -893,3 +893,20 @@ def test_engine_bounded_cache_needs_no_copy_of_a_long_prompt_per_sample(device):
         return _generate(e, prompts=[LONG_PROMPT, LONG_PROMPT[:5]], n=6, new=12, temperature=1.0), e.evictions
 
     assert run(25 + 12 * 6 + 1) == run(600)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_engine_evicts_in_groups_that_the_free_blocks_allow(device):
+    """Three samples grow to 6 blocks each and are cut back to 4 in the same step: with 4 blocks free one after the other, as the
+    blocks that one gives back serve the next."""
+    model = _debug_model(BF16 if device == "cuda" else FP32, device)
+    kw = {"cache_budget": 16, "cache_recent": 4, "cache_slack": 6}
+
+    def run(num_blocks):
+        e = _engine_of(model, num_blocks, **kw)
+        return _generate(e, prompts=[LONG_PROMPT[:22]], n=3, new=20, temperature=1.0), e.evictions
+
+    # 22 tokens at the 1st, 7th, 13th and 19th of 19 steps: each cuts back to 16, and six more make 22 again
+    assert run(3 * 6 + 4) == run(600) and run(600)[1] == 3 * 4
+    with pytest.raises(RuntimeError, match="exhausted"):
+        run(3 * 6 + 3)

@@ -358,11 +358,16 @@ class GenerationEngine:
         return self.cache_budget is not None and length >= self.cache_budget + self.cache_slack
 
     def _evict(self, seqs: list[_Seq]) -> None:
-        """Cut the caches of ``seqs`` back to the budget, layer by layer, into new blocks; the old ones are released."""
-        if not seqs:
-            return
-        dev, bs = self.device, self.block_size
-        need = -(-self.cache_budget // bs)
+        """Cut the caches of ``seqs`` back to the budget, layer by layer, into new blocks; the old ones are released. As many
+        sequences at a time as the free blocks hold: what they give back serves the next."""
+        need = -(-self.cache_budget // self.block_size) if seqs else 0
+        while seqs:
+            group = max(1, self.cache.alloc.available // need)
+            self._evict_group(seqs[:group], need)
+            seqs = seqs[group:]
+
+    def _evict_group(self, seqs: list[_Seq], need: int) -> None:
+        dev = self.device
         new: list[list[int]] = []
         try:
             for _ in seqs:
