@@ -910,3 +910,39 @@ def test_engine_evicts_in_groups_that_the_free_blocks_allow(device):
     assert run(3 * 6 + 4) == run(600) and run(600)[1] == 3 * 4
     with pytest.raises(RuntimeError, match="exhausted"):
         run(3 * 6 + 3)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("where", ["prefill", "fork", "decode", "evict"])
+def test_engine_returns_every_block_when_a_step_fails(where, device, monkeypatch):
+    """An exception anywhere in a run (as where memory runs out) leaves all blocks free."""
+    e = _engine(_debug_model(BF16 if device == "cuda" else FP32, device), cache_budget=16, cache_recent=4, cache_slack=6)
+    forward, evict, calls = e._forward, serving.kv_cache_evict, []
+
+    class Failed(Exception):
+        pass
+
+    def fail_forward(tokens, positions, meta, last_index=None):
+        if meta["prefill"] == (where == "prefill"):
+            raise Failed
+        return forward(tokens, positions, meta, last_index)
+
+    def fail_evict(*args):
+        calls.append(1)
+        if len(calls) == 2:                        # the second layer's
+            raise Failed
+        return evict(*args)
+
+    def fail_copy(src, dst):
+        raise Failed
+
+    if where in ("prefill", "decode"):
+        e._forward = fail_forward
+    elif where == "fork":
+        e.cache.copy_block = fail_copy
+    else:
+        monkeypatch.setattr(serving, "kv_cache_evict", fail_evict)
+    free = e.cache.alloc.available
+    with pytest.raises(Failed):
+        e.generate([LONG_PROMPT, LONG_PROMPT[:6]], n_samples=2, max_tokens=4, temperature=0.0, top_p=1.0)
+    assert e.cache.alloc.available == free == e.cache.num_blocks and not any(e.cache.alloc.refs)

@@ -256,12 +256,14 @@ class GenerationEngine:
         dev, bs = self.device, self.block_size
         shaper = _LogitShaper(prompts, n_samples, max_tokens, repetition_penalty, presence_penalty, frequency_penalty, logit_bias,
                               grammar, dev)
+        prompt_blocks: list[list[int]] = []
+        scratch: list[int] = []
+        seqs: list[_Seq] = []
         was_training = self.model.training
         self.model.eval()
         try:
             # -- prefill: all prompts packed in one row -------------------------------------------------
             toks, pos, doc, slots, last = [], [], [], [], []
-            prompt_blocks = []
             for i, p in enumerate(prompts):
                 nblk = (len(p) + bs - 1) // bs
                 blks: list[int] = []
@@ -275,13 +277,12 @@ class GenerationEngine:
                 last.append(len(toks) - 1)
             T = len(toks)
             pad = -T % 128 if dev.type == "cuda" else 0      # the flash kernel works on 128-token tiles
-            scratch = None
             if pad:
-                scratch = self.cache.alloc.alloc()            # padded tokens write into a throw-away block
+                scratch.append(self.cache.alloc.alloc())      # padded tokens write into a throw-away block
                 toks += [0] * pad
                 pos += range(pad)
                 doc += [len(prompts)] * pad
-                slots += [scratch * bs + (t % bs) for t in range(pad)]
+                slots += [scratch[0] * bs + (t % bs) for t in range(pad)]
             t_ = lambda x, dt: torch.tensor(x, dtype=dt, device=dev)  # noqa: E731
             if self.cache.scores is not None:
                 self.cache.clear_scores([b for blks in prompt_blocks for b in blks])
@@ -294,11 +295,10 @@ class GenerationEngine:
                                    for back in reversed(range(min(_OBSERVED, max(len(p) for p in prompts))))]
             logits = self._forward(t_(toks, torch.long).unsqueeze(0), t_(pos, torch.int32).unsqueeze(0), meta,
                                    last_index=t_(last, torch.long))
-            if scratch is not None:
-                self.cache.alloc.release(scratch)
+            while scratch:
+                self.cache.alloc.release(scratch.pop())
 
             # -- fork samples: share full prompt blocks, copy the partial tail ----------------------------
-            seqs: list[_Seq] = []
             for i, p in enumerate(prompts):
                 # weights are a sequence's own: no shared blocks, but for those of a prompt that the first decode step cuts back
                 # into every sample's own before anything is written
@@ -307,9 +307,8 @@ class GenerationEngine:
                     blks = [self.cache.alloc.share(b) for b in prompt_blocks[i][:full]]
                     seqs.append(_Seq(prompt=i, blocks=blks, length=len(p), position=len(p), tokens=[], logprobs=[]))
                     for src in prompt_blocks[i][full:]:
-                        nb = self.cache.alloc.alloc()
-                        self.cache.copy_block(src, nb)
-                        blks.append(nb)
+                        blks.append(self.cache.alloc.alloc())
+                        self.cache.copy_block(src, blks[-1])
                 while prompt_blocks[i]:
                     self.cache.alloc.release(prompt_blocks[i].pop())
             first_logits = logits.repeat_interleave(n_samples, dim=0)
@@ -344,11 +343,11 @@ class GenerationEngine:
                 cur_logits = self._decode_step(seqs, active, [t for _, t in nxt])
             return seqs
         finally:
-            for s in locals().get("seqs", []):
+            for s in seqs:
                 for b in s.blocks:
                     self.cache.alloc.release(b)
                 s.blocks = []
-            for blks in locals().get("prompt_blocks", []):      # a step above raised before the samples took over
+            for blks in (*prompt_blocks, scratch):      # not empty where a step above raised before the samples took over
                 for b in blks:
                     self.cache.alloc.release(b)
             if was_training:
@@ -374,18 +373,18 @@ class GenerationEngine:
                 new.append([])
                 for _ in range(need):
                     new[-1].append(self.cache.alloc.alloc())
-        except RuntimeError:
+            self.cache.clear_scores([b for blks in new for b in blks])
+            width = max(len(s.blocks) for s in seqs)
+            old_t = torch.tensor([s.blocks + [0] * (width - len(s.blocks)) for s in seqs], dtype=torch.int32, device=dev)
+            lens = torch.tensor([s.length for s in seqs], dtype=torch.int32, device=dev)
+            new_t = torch.tensor(new, dtype=torch.int32, device=dev)
+            for k, v, scores in zip(self.cache.k, self.cache.v, self.cache.scores):
+                serving.kv_cache_evict(k, v, scores, old_t, lens, new_t, self.cache_budget, self.cache_recent)
+        except BaseException:
             for blks in new:
                 for b in blks:
                     self.cache.alloc.release(b)
             raise
-        self.cache.clear_scores([b for blks in new for b in blks])
-        width = max(len(s.blocks) for s in seqs)
-        old_t = torch.tensor([s.blocks + [0] * (width - len(s.blocks)) for s in seqs], dtype=torch.int32, device=dev)
-        lens = torch.tensor([s.length for s in seqs], dtype=torch.int32, device=dev)
-        new_t = torch.tensor(new, dtype=torch.int32, device=dev)
-        for k, v, scores in zip(self.cache.k, self.cache.v, self.cache.scores):
-            serving.kv_cache_evict(k, v, scores, old_t, lens, new_t, self.cache_budget, self.cache_recent)
         for s, blks in zip(seqs, new):
             for b in s.blocks:
                 self.cache.alloc.release(b)
