@@ -6,7 +6,7 @@ import torch
 
 from test_decode_ops import BF16, FP16, attention_oracle, check_attention, make_cache, rows_of
 
-from torchtitan_b200.ops import serving
+from torchtitan_b200.ops import cuda_ops, serving
 
 pytestmark = pytest.mark.gpu
 
@@ -348,3 +348,27 @@ def test_whole_numbers_past_32_bits_are_outside(value):
         want[0, [5, 6]] -= 0.5
         want[1, 7] -= 1.0
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("sinks", [False, True])
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, BF16), (256, FP16)])
+def test_join_by_warps(D, dtype, sinks):
+    """Enough heads for a warp to join each, up to 32 chunks: the bits of every sequence by itself, which a block joins -- of its
+    weights too, which show a last bit of the denominator that the output's rounding hides."""
+    lens = [16_384, 0, 1, 600, 5000, 1024, 1025, 12_345] + [1100 + 7 * i for i in range(12)]
+    H, hkv = 64, 4
+    assert len(lens) * H >= 1184
+    k, v, table, n, _ = make_cache(lens, hkv=hkv, dim=D, page=32, dtype=dtype, device="cuda", seed=D)
+    for seed in range(10):
+        torch.manual_seed(seed)
+        q = torch.randn(len(lens), H, D, device="cuda").to(dtype)
+        sink = torch.randn(H, device="cuda") if sinks else None
+        scores, alone = torch.zeros(k.shape[0], hkv, 32, device="cuda"), torch.zeros(k.shape[0], hkv, 32, device="cuda")
+        out, lse = _attend(q, k, v, table, n, sinks=sink, scores=scores, return_lse=True)
+        for b in range(len(lens)):
+            one, l1 = _attend(q[b : b + 1], k, v, table[b : b + 1], n[b : b + 1], sinks=sink, scores=alone, return_lse=True)
+            assert torch.equal(one[0], out[b]) and torch.equal(l1[0], lse[b])
+        assert torch.equal(scores, alone)
+    short = [3, 5, 6]
+    oracle = attention_oracle(q[short], k, v, table[short], n[short], D**-0.5, sinks=sink)
+    check_attention(out[short], oracle, 512 + 4 + 256, D, dtype, lse[short])

@@ -128,21 +128,22 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v)
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 
 // The end of a query head: sink, division, output of dims d and d + 1. top, sum, x: maximum, sum and weighted values over all
-// of its tokens.
+// of its tokens. Three kernels end in it, and a sequence must get the same bits from each: products and sums are rounded on
+// their own here and in the joins' sums, not left to the compiler to contract in one kernel and not in another.
 template <typename T, int D>
 __device__ __forceinline__ void finish(const Args& a, int b, int h, int d, float top, float sum, float2 x) {
   const long long bh = static_cast<long long>(b) * a.H + h;
   if (a.sinks) {
-    const float sink = a.sinks[h] * kLog2e, all = fmaxf(top, sink), base = all == -INFINITY ? 0.f : all;
-    const float f = exp2f(top - base);
-    x.x *= f;
-    x.y *= f;
-    sum = sum * f + (sink == all && all != -INFINITY ? 1.f : exp2f(sink - base));
+    const float sink = __fmul_rn(a.sinks[h], kLog2e), all = fmaxf(top, sink), base = all == -INFINITY ? 0.f : all;
+    const float f = exp2f(__fsub_rn(top, base));
+    x.x = __fmul_rn(x.x, f);
+    x.y = __fmul_rn(x.y, f);
+    sum = __fadd_rn(__fmul_rn(sum, f), sink == all && all != -INFINITY ? 1.f : exp2f(__fsub_rn(sink, base)));
     top = all;
   }
   *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + bh * D + d) = sum == 0.f ? 0u : pack2<T>(x.x / sum, x.y / sum);
   if (d == 0) {
-    if (a.lse) a.lse[bh] = (top + log2f(sum)) * kLn2;
+    if (a.lse) a.lse[bh] = __fmul_rn(__fadd_rn(top, log2f(sum)), kLn2);
     if (a.ws_tot) a.ws_tot[bh] = make_float2(top, sum);
   }
 }
@@ -626,9 +627,9 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Args a) {
     if (w < warps) top = fmaxf(top, s_top[w]);
   const float f = ex2(mine.x - (top == -INFINITY ? 0.f : top));
   if (tid < nc) s_f[tid] = f;
-  float sum = tid < nc ? mine.y * f : 0.f;
+  float sum = tid < nc ? __fmul_rn(mine.y, f) : 0.f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int o = 16; o > 0; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
   if (lane == 0) s_sum[warp] = sum;
   __syncthreads();
   float x[V] = {};
@@ -649,13 +650,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Args a) {
     sum = r.bad ? NAN : 0.f;
 #pragma unroll
     for (int w = 0; w < kMaxChunks / 32; ++w)
-      if (w < warps) sum += s_sum[w];
+      if (w < warps) sum = __fadd_rn(sum, s_sum[w]);
     float2 all = *reinterpret_cast<const float2*>(s_x[0] + 2 * tid);
 #pragma unroll 8
     for (int w = 1; w < warps; ++w) {
       const float2 u = *reinterpret_cast<const float2*>(s_x[w] + 2 * tid);
-      all.x += u.x;
-      all.y += u.y;
+      all.x = __fadd_rn(all.x, u.x);
+      all.y = __fadd_rn(all.y, u.y);
     }
     finish<T, D>(a, b, h, 2 * tid, top, sum, all);
   }
@@ -685,9 +686,9 @@ __global__ void __launch_bounds__(kFewThreads) join_few_kernel(const Args a) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float f = ex2(mine.x - (top == -INFINITY ? 0.f : top));
-  float sum = lane < nc ? mine.y * f : 0.f;
+  float sum = lane < nc ? __fmul_rn(mine.y, f) : 0.f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int o = 16; o > 0; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
   if (r.bad) sum = NAN;
   float all[V] = {};
   for (int c0 = 0; c0 < nc; c0 += kAhead) {
