@@ -350,6 +350,36 @@ def test_whole_numbers_past_32_bits_are_outside(value):
     assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("past", [-1, 0, 1, 70_000])
+def test_where_chunks_begin_to_grow(past):
+    """Sequences around the length from which chunks are longer than the least, with a short one beside them. A term passes at
+    most chunk + 4 + 256 additions (its chunk's, the groups', the join's), so errors are bounded by that many, not by the tokens:
+    a chunk left out of a sum would show."""
+    least, most = cuda_ops._split_rule()
+    n = least * most + past
+    k, v, table, lens, _ = make_cache([n, 700], hkv=2, dim=64, page=64, dtype=FP16, device="cuda", seed=past)
+    for b, m in enumerate((n, 700)):
+        v[table[b, : -(-m // 64)].long()] += 3.0                  # what is missing does not average out
+    q = torch.randn(2, 4, 64, device="cuda").to(FP16)
+    scores = torch.zeros(k.shape[0], 2, 64, device="cuda")
+    out, lse = _attend(q, k, v, table, lens, scores=scores, return_lse=True)
+    oracle = attention_oracle(q, k, v, table, lens, 0.125)
+    check_attention(out, oracle, 2 * least + 4 + most, 64, FP16, lse, scores, torch.zeros_like(scores), table)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_join_of_more_chunks_than_one_pass_holds(D):
+    """137 chunks: with 256 dims more than 32 warps fetch at once."""
+    n = 70_000
+    k, v, table, lens, _ = make_cache([n, 33], hkv=1, dim=D, page=128, dtype=FP16, device="cuda", seed=D)
+    for b, m in enumerate((n, 33)):
+        v[table[b, : -(-m // 128)].long()] += 3.0
+    q = torch.randn(2, 2, D, device="cuda").to(FP16)
+    scores = torch.zeros(k.shape[0], 1, 128, device="cuda")
+    out, lse = _attend(q, k, v, table, lens, scores=scores, return_lse=True)
+    check_attention(out, attention_oracle(q, k, v, table, lens, D**-0.5), 512 + 4 + 256, D, FP16, lse, scores, torch.zeros_like(scores), table)
+
+
 @pytest.mark.parametrize("sinks", [False, True])
 @pytest.mark.parametrize("D,dtype", [(64, BF16), (128, BF16), (256, FP16)])
 def test_join_by_warps(D, dtype, sinks):
@@ -372,3 +402,15 @@ def test_join_by_warps(D, dtype, sinks):
     short = [3, 5, 6]
     oracle = attention_oracle(q[short], k, v, table[short], n[short], D**-0.5, sinks=sink)
     check_attention(out[short], oracle, 512 + 4 + 256, D, dtype, lse[short])
+
+
+@pytest.mark.parametrize("G,D", [(72, 64), (130, 128), (65, 64)])
+def test_many_query_heads_to_a_kv_head(G, D):
+    """Weights are summed 64 query heads at a time."""
+    lens = [1500, 3, 0, 64]
+    k, v, table, n, _ = make_cache(lens, hkv=2, dim=D, page=16, dtype=BF16, device="cuda", seed=G)
+    q = torch.randn(len(lens), 2 * G, D, device="cuda").to(BF16)
+    scores = torch.rand(k.shape[0], 2, 16, device="cuda")
+    before = scores.clone()
+    out, lse = _attend(q, k, v, table, n, scores=scores, return_lse=True)
+    check_attention(out, attention_oracle(q, k, v, table, n, D**-0.5), max(lens), D, BF16, lse, scores, before, table)

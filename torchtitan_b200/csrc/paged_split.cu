@@ -709,7 +709,8 @@ __global__ void __launch_bounds__(kFewThreads) join_few_kernel(const Args a) {
 }
 
 // CTA = (chunk, kv head, sequence): a token's weights over the query heads of its kv head, added to its score. One addition
-// per page slot and sequence, atomic only because two sequences may share a page.
+// per page slot and sequence for every 64 query heads of the kv head, in their order (the same thread adds them); atomic only
+// because two sequences may share a page.
 __global__ void __launch_bounds__(512) score_kernel(const Args a) {
   const int c = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, G = a.H / a.Hkv, tid = threadIdx.x;
   const Range r = range_of(a, b);
