@@ -946,3 +946,46 @@ def test_engine_returns_every_block_when_a_step_fails(where, device, monkeypatch
     with pytest.raises(Failed):
         e.generate([LONG_PROMPT, LONG_PROMPT[:6]], n_samples=2, max_tokens=4, temperature=0.0, top_p=1.0)
     assert e.cache.alloc.available == free == e.cache.num_blocks and not any(e.cache.alloc.refs)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kw", [{}, {"cache_budget": 16, "cache_recent": 4, "cache_slack": 6}])
+def test_engine_refuses_positions_past_the_rotary_table(kw, device):
+    """A bounded cache never fills up, so the table of 512 positions is what ends a sequence: its rows are read by position."""
+    model = _debug_model(BF16 if device == "cuda" else FP32, device)
+    prompt = [(5 * i) % 300 + 1 for i in range(500)]
+    e = _engine(model, **kw)
+    tokens, _ = _generate(e, prompts=[prompt, prompt[:9]], n=1, new=13)       # positions 500 ... 511
+    assert [len(t) for t in tokens] == [13, 13]
+    for prompts, new in (([prompt[:9], prompt], 14), ([prompt + prompt[:13]], 1)):
+        with pytest.raises(ValueError, match="position 512"):
+            e.generate(prompts, n_samples=1, max_tokens=new, temperature=0.0, top_p=1.0)
+        assert e.cache.alloc.available == e.cache.num_blocks
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_engine_with_a_short_rotary_table(device):
+    """A table shorter than the padding of a prefill on the GPU (up to 127 tokens)."""
+    import dataclasses
+
+    from torchtitan_b200.models.qwen3 import model_registry
+
+    cfg = dataclasses.replace(model_registry("debugmodel").model, n_layers=2)
+    seen = []
+    for rows in (40, 512):
+        cfg.rope = dataclasses.replace(cfg.rope, max_seq_len=rows)
+        torch.manual_seed(0)
+        model = cfg.build().to(dtype=BF16 if device == "cuda" else FP32, device=device)
+        with torch.no_grad():
+            model.init_weights(buffer_device=torch.device(device))
+        e = _engine(model)
+        forward, past = e._forward, []
+
+        def spy(tokens, positions, meta, last_index=None, forward=forward, past=past):
+            past.append(int(positions.max()))
+            return forward(tokens, positions, meta, last_index)
+
+        e._forward = spy
+        seen.append(_generate(e, n=1, new=4))
+        assert rows > 40 or max(past) < rows
+    assert seen[0] == seen[1]

@@ -15,10 +15,10 @@ once in a CUDA graph and replayed (inputs live in static buffers), removing per-
 For long generations, ``split_decode=True`` decodes with attention split over the cache's length, and ``cache_budget``
 bounds the tokens that a sequence keeps in the cache: attention weights are accumulated per cached token, and a sequence
 that outgrows the budget by ``cache_slack`` is cut back to its most attended tokens (per layer and kv head). Positions go on
-counting; the sequence's pages are its own, shared with the prompt's other samples only until the first step cuts a prompt
-that outgrows the budget back. Both keep a sequence's result independent of the batch it runs in. Penalties, biases and a
-grammar change what is drawn; the reported log-probabilities stay those of the model's own logits, which is what the trainer
-recomputes.
+counting, up to the rows of the model's rotary table; the sequence's pages are its own, shared with the prompt's other samples
+only until the first step cuts a prompt that outgrows the budget back. Both keep a sequence's result independent of the batch
+it runs in. Penalties, biases and a grammar change what is drawn; the reported log-probabilities stay those of the model's own
+logits, which is what the trainer recomputes.
 """
 
 from __future__ import annotations
@@ -202,6 +202,11 @@ class GenerationEngine:
         self.decode_steps = 0
         self.weight_half = 0   # which half of a double-buffered parameter arena the model currently reads
 
+    def _check_position(self, position: int) -> None:
+        """Rows of the rotary table are read by position, on the GPU without a check."""
+        if position >= (rows := self.model.freqs_cis.shape[0]):
+            raise ValueError(f"position {rows} is past the model's rotary table (max_seq_len {rows}): shorten the prompt or max_tokens")
+
     # ---- one pass over the blocks with cache reads/writes -----------------------------------------
     def _attention(self, att, x, positions, layer: int, meta):
         T = x.shape[1]
@@ -265,6 +270,7 @@ class GenerationEngine:
             # -- prefill: all prompts packed in one row -------------------------------------------------
             toks, pos, doc, slots, last = [], [], [], [], []
             for i, p in enumerate(prompts):
+                self._check_position(len(p) - 1)
                 nblk = (len(p) + bs - 1) // bs
                 blks: list[int] = []
                 prompt_blocks.append(blks)
@@ -280,7 +286,7 @@ class GenerationEngine:
             if pad:
                 scratch.append(self.cache.alloc.alloc())      # padded tokens write into a throw-away block
                 toks += [0] * pad
-                pos += range(pad)
+                pos += [t % self.model.freqs_cis.shape[0] for t in range(pad)]
                 doc += [len(prompts)] * pad
                 slots += [scratch[0] * bs + (t % bs) for t in range(pad)]
             t_ = lambda x, dt: torch.tensor(x, dtype=dt, device=dev)  # noqa: E731
@@ -398,6 +404,7 @@ class GenerationEngine:
         self._evict([seqs[si] for si in active if self._outgrown(seqs[si].length)])
         for si in active:
             s = seqs[si]
+            self._check_position(s.position)
             if s.length % bs == 0 and s.length // bs >= len(s.blocks):
                 s.blocks.append(self.cache.alloc.alloc())
                 handed_out.append(s.blocks[-1])
