@@ -158,7 +158,7 @@ __device__ __forceinline__ void select_rows(const Args& a, int b, int h, int par
       }
     }
   } else {
-    for (int i0 = tid; i0 < count; i0 += kAhead * kThreads) {     
+    for (int i0 = tid; i0 < count; i0 += kAhead * kThreads) {
       int page[kAhead], slot[kAhead];
       uint32_t k[kAhead];
 #pragma unroll
@@ -262,7 +262,7 @@ __device__ __forceinline__ void select_rows(const Args& a, int b, int h, int par
       }
       above += c[e];
     }
-    // the histogram of the round after next; the others are done with the one of the round before this one
+    // the next round's histogram: the others were done with it when they came to this round's meeting
     for (int i = tid; i < kBins; i += kThreads) hist[(round + 1) & 1][i] = 0;
     __syncthreads();
     lo += static_cast<uint32_t>(s_bin) << shift;
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kMoveThreads, 12) move_kernel(const Args a) {
 }
 
 // Small caches in one launch, as launches are most of their time: cluster = (kv head, sequence), its first CTA selects, all move.
-// 1056 tokens, 8 kv heads, keep 1024: 17.8 us a call against 20.4 with two launches (9.3 against 8.4 in a captured graph); with 512
+// 1056 tokens, 8 kv heads, keep 1024: 18 us a call against 20.4 with two launches (9.5 against 8.4 in a captured graph); with 512
 // threads 10.1, with clusters of 4 14.6.
 constexpr int kSmallRoom = 8192, kSmallBytes = 128 << 10;     // tokens of a table; kept keys and values to a CTA
 

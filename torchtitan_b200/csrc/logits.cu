@@ -16,8 +16,10 @@
 // streams its part, 16 bytes to a thread, which the L2 has fetched meanwhile.
 //
 // What bounds it: each logit is read and written once. 256 rows of 151936 fp32 logits with 2048 tokens of history, 32 biases and
-// a mask: 62.6 us, 5.1 TB/s, 0.77 of the measured copy rate; with a mask and one token of history 52 us. Parts of 12288 logits, four blocks of 512
-// threads to an SM: with 6144 more of the time goes to the histories (74 us against 67), with 20480 fewer blocks overlap.
+// a mask: 63 us, 5.1 TB/s, 0.77 of the measured copy rate; with a mask and one token of history 52 us. Parts of 12288 logits, four blocks of 512
+// threads to an SM: with 6144 more of the time goes to the histories (74 us against 67), with 20480 fewer blocks overlap. Where
+// blocks are few and histories long (24 rows of 50021 bf16 logits, 32768 tokens: 16 us in a graph, 1 us of bytes) a block has its SM
+// to itself, but still the registers and the two loads ahead of one that shares it: 27 % of a warp's time is waiting for tokens.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -186,7 +188,8 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_kernel(const Args a) {
     if constexpr (WORDS) f = adjust(f, word[pad + i - v0], set, s_sum);
     y[i] = mask && !((mask[i / 32] >> (i % 32)) & 1u) ? from_f<T>(-INFINITY) : (WORDS ? from_f<T>(f) : x[i]);
   };
-  // vectors where x and y lie alike, single logits before and behind them (and everywhere otherwise)
+  // vectors where x and y lie alike, single logits before and behind them (and everywhere otherwise: 256 rows of 151937 fp32 logits
+  // out of padded rows into dense ones 96 us, into rows padded alike 60)
   const bool alike = reinterpret_cast<uintptr_t>(x) % 16 == reinterpret_cast<uintptr_t>(y) % 16;
   const int w0 = alike ? min(v1, v0 + head) : v1, w1 = w0 + (v1 - w0) / E * E;
   for (int i = v0 + tid; i < w0; i += kThreads) one(i);

@@ -21,9 +21,12 @@
 // stopped at 3.5 TB/s; copies with the address of every row looked up, at 3.6.
 // Chunks of 512 tokens: with 256 the partial results and meetings cost 128 sequences up to 8192 (16/8 heads) 375 us against
 // 353, with 1024 a ragged batch is left waiting for its last chunks (64 sequences up to 4096, 32/4 heads: 99 us against 81).
-// Measured (B200, calls back to back): 128 sequences up to 8192 tokens, 16/8 heads of 128: 370 to 385 us, 5.6 to 5.9 TB/s, 0.86 to
-// 0.89 of the measured copy rate; one of 131072, 32/8 heads: 99 us, 5.4 TB/s; 64 up to 4096, 32/4 heads, with scores: 72 us, 3.9
-// TB/s. With the products left out 32 of 8192 and one of 131072 take the same time.
+// Measured (several B200s, calls back to back): 128 sequences up to 8192 tokens, 16/8 heads of 128: 363 to 385 us, 5.6 to 6.0 TB/s,
+// 0.86 to 0.91 of the measured copy rate; one of 131072, 32/8 heads: 99 to 103 us, 5.2 to 5.4 TB/s; 64 up to 4096, 32/4 heads, with
+// scores: 72 us, 3.9 TB/s. With the products left out 32 of 8192 and one of 131072 take the same time.
+// Not bound by memory: 256 dims with 16 query heads to a kv head (6 of 5003, fp16: 45 us in a graph, 19 us of bytes). One CTA of
+// eight warps fills an SM, the busiest has 1024 tokens where the mean is 811, and a warp spends 32 % of its time on fixed
+// latencies, 16 % on tokens, 11 % on meetings: the dependent products, exchange and transposes of every 16 tokens.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
