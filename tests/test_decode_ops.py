@@ -836,15 +836,16 @@ def test_evict_does_not_look_at_table_entries_behind_a_sequence(beyond, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
-def test_evict_refuses_a_keep_past_31_bits(device):
-    """Kept tokens are counted in 32 bits: 2^32 + 5 must not become 5 (an empty batch, as `kept` has `keep` columns)."""
+def test_evict_refuses_a_keep_of_2_to_the_30(device):
+    """Kept tokens are counted in 32 bits, in steps of thousands: 2^32 + 5 must not become 5, nor a loop pass 2^31 (an empty batch,
+    as `kept` has `keep` columns)."""
     k, v, table, n, free = make_cache([40], hkv=2, dim=64, page=16, dtype=BF16, device=device, spare=8)
     s, fresh = torch.zeros(k.shape[0], 2, 16, device=device), free[:4].view(1, 4).to(device)
-    for keep in (1 << 31, (1 << 32) + 5):
+    for keep in (1 << 30, (1 << 31) - 1, 1 << 31, (1 << 32) + 5):
         with pytest.raises(ValueError, match="keep"):
             serving.kv_cache_evict(k, v, s, table[:0], n[:0], fresh[:0], keep)
-    lens, kept = serving.kv_cache_evict(k, v, s, table[:0], n[:0], fresh[:0], (1 << 31) - 1)
-    assert lens.shape == (0,) and kept.shape == (0, 2, (1 << 31) - 1)
+    lens, kept = serving.kv_cache_evict(k, v, s, table[:0], n[:0], fresh[:0], (1 << 30) - 1)
+    assert lens.shape == (0,) and kept.shape == (0, 2, (1 << 30) - 1)
 
 
 @pytest.mark.parametrize("device", DEVICES)

@@ -212,8 +212,8 @@ def kv_cache_evict(k_cache, v_cache, scores, block_tables, context_lens, new_tab
     B = block_tables.shape[0]
     _check_cache(k_cache, v_cache, scores, block_tables, context_lens, B)
     nb, bs, hkv, D = k_cache.shape
-    if not isinstance(keep, int) or not isinstance(recent, int) or not 1 <= keep < 1 << 31 or not 0 <= recent <= keep:
-        raise ValueError(f"keep must be a whole number in [1, 2^31) and recent one in [0, keep], got {keep} and {recent}")
+    if not isinstance(keep, int) or not isinstance(recent, int) or not 1 <= keep < 1 << 30 or not 0 <= recent <= keep:
+        raise ValueError(f"keep must be a whole number in [1, 2^30) and recent one in [0, keep], got {keep} and {recent}")
     _whole_numbers(new_tables, "new_tables", B, 2, k_cache.device)
     room = block_tables.shape[1] * bs
     most = min(keep, room)
